@@ -104,6 +104,94 @@ s2p_status s2p_b200_attention_decode_noalloc(const s2p_bf16* q, const s2p_bf16* 
                                              s2p_bf16* out, int q_heads, int kv_heads, int head_dim, int pos,
                                              int max_seq, cudaStream_t stream);
 
+/* ===== paged 4-bit cache (no counterpart in the reference, whose sessions own contiguous bf16 or INT8 planes) =====
+ *
+ * Keys and values of many sequences in pages of 64 positions, 4 bits a channel, with what writes them, what attends over
+ * them and what moves their pages.  Sequences that begin alike (a voice's prompt) share pages instead of copying them.
+ *
+ * All state is the caller's, in device memory of the current device, and every call works in stream order on it without
+ * reading anything back, so a captured graph of reserve, append and attention calls replays as the sequences grow.  Calls
+ * that share a cache or a workspace must be ordered: on one stream, or by events.
+ *
+ * A pool is n_pages pages of s2p_b200_kv4_page_bytes() bytes: [layers][kv_heads][4 blocks of 16 positions][2560 bytes].
+ * In groups of 32 channels of one position a code c (0..15) stands for s c + m, with f16 m = the group's smallest value and
+ * f16 s = (largest - smallest) / 15 (each rounded to nearest), c = (x - m) / s rounded to the nearest, ties to even, kept in
+ * 0..15 (0 where s is 0).  Values beyond +-65504 are kept at that, a NaN takes code 0, and a group of nothing but NaN stands for zeros.
+ * Block of position p (p % 16 = i), byte offsets; channel d of group j = d / 32, e = d % 32; even d in the low four bits:
+ *   keys    codes       64 i + 16 (e / 8) + 4 j + (e % 8) / 2
+ *           s, m        2048 + 16 i + 2 j,  2056 + 16 i + 2 j
+ *   values  codes       1024 + 512 (i / 8) + 64 (e / 4) + 16 (i / 2 % 4) + 8 (i % 2) + 2 j + (e % 4) / 2
+ *           s, m        2304 + 16 (i / 2) + 4 j + 2 (i % 2),  2432 + the same
+ * (the order in which the matrix instructions of the attention take them: a lane's bytes lie together). */
+#define S2P_B200_KV4_PAGE 64
+#define S2P_B200_KV4_MAX_BATCH 1024 /* sequences of one batch */
+#define S2P_B200_KV4_MAX_LIST 256   /* sequences of one fork or release call */
+
+typedef struct {
+    void* pages;      /* the pool, 128-byte aligned */
+    int32_t* table;   /* [max_seqs][table_stride]: page of positions 64 j .. 64 j + 63; an entry outside the pool (-1) holds nothing */
+    int32_t* lens;    /* [max_seqs] positions held; table entries behind them are -1 */
+    int32_t* refs;    /* [n_pages] table entries that name the page; 0 = free */
+    void* work;       /* 256-byte aligned; zeroed once by the caller, every call leaves its first part zeroed again */
+    size_t work_bytes;
+    int n_pages, layers, kv_heads, q_heads; /* q_heads a multiple of kv_heads, at most 16 times as many; width 128 */
+    int max_seqs, table_stride;
+} s2p_b200_kv4;
+
+/* The rows of a tick or a prompt slice: entry b brings rows row0[b] .. row0[b + 1] - 1 of the activations, at positions
+ * pos0[b], pos0[b] + 1, ... of sequence seqs[b].  All arrays are device memory.  A sequence stands in a batch once; an entry
+ * may have no rows; entries whose pos0 is negative or beyond 2^30, or whose sequence is outside 0 .. max_seqs - 1, store
+ * nothing and see nothing, and zeros come out for their rows; rows behind row0[n] are left as they were. */
+typedef struct {
+    const int32_t* seqs; /* [n] */
+    const int32_t* row0; /* [n + 1], not decreasing */
+    int32_t* pos0;       /* [n], written by reserve */
+    int n;
+    int rows;     /* rows of the activations: those from row0[n] on are padding */
+    int max_rows; /* the most rows that an entry has; only the choice of kernels goes by it, so it may be more or less */
+} s2p_b200_kv4_batch;
+
+size_t s2p_b200_kv4_page_bytes(int layers, int kv_heads);
+/* workspace of every call on this cache, attention with batches of up to `rows` rows; 0 if the cache's sizes cannot be served */
+size_t s2p_b200_kv4_work_bytes(const s2p_b200_kv4* c, int rows);
+/* S2P_ERR_INTERNAL if a bounded wait of an earlier call on this workspace gave up (its rows are lost), once; waits for the stream */
+s2p_status s2p_b200_kv4_status(const s2p_b200_kv4* c, cudaStream_t stream);
+
+/* Room for the batch's rows: pos0 = positions held, lens += rows, and free pages (lowest first, in the batch's order) for
+ * what the last held page does not take.  An entry that needs more pages than are left after all before it, or more table
+ * entries than there are, is refused: pos0 = -1, and it keeps what it held.  info (device, may be NULL): pages free
+ * afterwards, entries refused. */
+s2p_status s2p_b200_kv4_reserve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int32_t* info, cudaStream_t stream);
+
+/* From raw rows qkv [rows, (q_heads + 2 kv_heads) * 128]: RMS norm of each query and key head (gains q_norm, k_norm [128];
+ * NULL: no norm), rotation of its channel pairs (2 i, 2 i + 1) by position * rope_base^(-2 i / 128), queries to q
+ * [rows, q_heads * 128], keys and values into the pages of `layer`.  In one pass and in 32 bits, the angle in 64: a query is
+ * rounded once, to bf16, a key only to its 4 bits.  (s2pk_rope rounds cosine and sine to bf16, as the reference does.)
+ * Rows whose position has no page come out in q all the same. */
+s2p_status s2p_b200_kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const s2p_bf16* qkv, const s2p_bf16* q_norm,
+                               const s2p_bf16* k_norm, float eps, float rope_base, s2p_bf16* q, cudaStream_t stream);
+
+/* out [rows, q_heads * 128]: softmax(q k / sqrt(128)) v over the positions of the row's sequence up to its own that have a
+ * page; zeros where there is none. */
+s2p_status s2p_b200_kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const s2p_bf16* q, s2p_bf16* out,
+                                  cudaStream_t stream);
+
+/* The values that the cache holds at the batch's positions, rounded to bf16: k and v [rows, kv_heads * 128], zeros where there is no page. */
+s2p_status s2p_b200_kv4_read(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, s2p_bf16* k, s2p_bf16* v, cudaStream_t stream);
+
+/* Sequences children[i] become the first tokens[i] positions of parents[i] (fewer if it holds fewer; -1: all).  What the
+ * children held is released first.  Full pages are shared; the last one, if it is not full, is copied into a free page
+ * (lowest first, in the list's order), so that a shared page is never written again.  Without a free page child i is left
+ * empty.  The lists are host memory, read before the call returns; a sequence stands among the children once and not among the
+ * parents as well (S2P_ERR_INVALID).  info as above. */
+s2p_status s2p_b200_kv4_fork(const s2p_b200_kv4* c, const int32_t* parents, const int32_t* children, const int32_t* tokens, int n,
+                             int32_t* info, cudaStream_t stream);
+/* Empties the sequences (host list, each once); pages that no other sequence holds become free. */
+s2p_status s2p_b200_kv4_release(const s2p_b200_kv4* c, const int32_t* seqs, int n, cudaStream_t stream);
+/* Moves pages until the used ones are the lowest: the k-th used page behind them to the k-th free one among them, with all
+ * layers, references and table entries.  info: pages free, pages moved. */
+s2p_status s2p_b200_kv4_compact(const s2p_b200_kv4* c, int32_t* info, cudaStream_t stream);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

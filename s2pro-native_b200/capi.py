@@ -122,6 +122,19 @@ class Stats(C.Structure):
                 ("last_tick_persistent", C.c_int)]
 
 
+class Kv4(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("table", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p),
+                ("work", C.c_void_p), ("work_bytes", C.c_size_t), ("n_pages", C.c_int), ("layers", C.c_int),
+                ("kv_heads", C.c_int), ("q_heads", C.c_int), ("max_seqs", C.c_int), ("table_stride", C.c_int)]
+
+
+class Kv4Batch(C.Structure):
+    _fields_ = [("seqs", C.c_void_p), ("row0", C.c_void_p), ("pos0", C.c_void_p), ("n", C.c_int), ("rows", C.c_int),
+                ("max_rows", C.c_int)]
+
+
+_KV4, _KV4B = C.POINTER(Kv4), C.POINTER(Kv4Batch)
+
 EXT_PROTOTYPES = {
     "s2p_b200_version": (C.c_char_p, []),
     "s2p_b200_model_stats": (_I, [_P, C.POINTER(Stats)]),
@@ -131,6 +144,16 @@ EXT_PROTOTYPES = {
     "s2p_b200_model_tp_export": (_I, [_P, _P]),
     "s2p_b200_model_tp_attach": (_I, [_P, _I, _I, _P]),
     "s2p_b200_attention_decode_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _S]),
+    "s2p_b200_kv4_page_bytes": (C.c_size_t, [_I, _I]),
+    "s2p_b200_kv4_work_bytes": (C.c_size_t, [_KV4, _I]),
+    "s2p_b200_kv4_status": (_I, [_KV4, _S]),
+    "s2p_b200_kv4_reserve": (_I, [_KV4, _KV4B, _P, _S]),
+    "s2p_b200_kv4_append": (_I, [_KV4, _KV4B, _I, _P, _P, _P, C.c_float, C.c_float, _P, _S]),
+    "s2p_b200_kv4_attention": (_I, [_KV4, _KV4B, _I, _P, _P, _S]),
+    "s2p_b200_kv4_read": (_I, [_KV4, _KV4B, _I, _P, _P, _S]),
+    "s2p_b200_kv4_fork": (_I, [_KV4, _P, _P, _P, _I, _P, _S]),
+    "s2p_b200_kv4_release": (_I, [_KV4, _P, _I, _S]),
+    "s2p_b200_kv4_compact": (_I, [_KV4, _P, _S]),
 }
 
 
