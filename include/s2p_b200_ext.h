@@ -132,7 +132,7 @@ typedef struct {
     int32_t* table;   /* [max_seqs][table_stride]: page of positions 64 j .. 64 j + 63; an entry outside the pool (-1) holds nothing */
     int32_t* lens;    /* [max_seqs] positions held; table entries behind them are -1 */
     int32_t* refs;    /* [n_pages] table entries that name the page; 0 = free */
-    void* work;       /* 256-byte aligned; zeroed once by the caller, every call leaves its first part zeroed again */
+    void* work;       /* 256-byte aligned; zeroed once by the caller, before its first use */
     size_t work_bytes;
     int n_pages, layers, kv_heads, q_heads; /* q_heads a multiple of kv_heads, at most 16 times as many; width 128 */
     int max_seqs, table_stride;
@@ -172,7 +172,7 @@ s2p_status s2p_b200_kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
                                const s2p_bf16* k_norm, float eps, float rope_base, s2p_bf16* q, cudaStream_t stream);
 
 /* out [rows, q_heads * 128]: softmax(q k / sqrt(128)) v over the positions of the row's sequence up to its own that have a
- * page; zeros where there is none. */
+ * page; zeros where there is none.  rows * kv_heads * table_stride is at most 2^29. */
 s2p_status s2p_b200_kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const s2p_bf16* q, s2p_bf16* out,
                                   cudaStream_t stream);
 

@@ -10,20 +10,28 @@
 #define KV4_HEAD_BYTES (4 * KV4_BLOCK_BYTES)
 #define KV4_MAX_GROUP 16         /* query heads of a kv head */
 #define KV4_MAX_STRIDE (1 << 24) /* table entries of a sequence: positions stay below 2^30 */
+#define KV4_MAX_LINE (1 << 29)   /* rows * kv_heads * table_stride of an attention call: its blocks are counted in 32 bits */
 
-/* The workspace: status word | arrival counters of the split attention, zero between calls | one area for either the partials
- * of a split attention or the lists of the page operators. */
-#define KV4_MAX_CTAS 320         /* CTAs that may leave partials, two each */
-#define KV4_PART_COLS 16         /* (row, head) columns of a partial */
-#define KV4_PART_FLOATS (KV4_PART_COLS * (128 + 2))
+/* The workspace: status word | one area for either the partials of a split attention or the lists of the page operators |
+ * arrival counters of the split attention, zero between calls.  Only the last part's size goes by the rows, so that calls
+ * with different numbers of rows agree on where everything is. */
 #define KV4_STATUS_BYTES 256
+#define KV4_PARTS (2 * 320 * 8 * 8) /* columns of partials: two for each of 8 columns of 8 warps of up to 320 CTAs; 128 + 2 floats each */
 
 #ifdef __cplusplus
 namespace s2p {
 extern "C" {
 #endif
 
-size_t kv4_counter_bytes(int rows, int kv_heads);
+/* Bytes of the area.  The page operators keep a few words, a pair of pages per move and a new number per page. */
+static inline size_t kv4_area_bytes(int n_pages) {
+    const size_t part = (size_t)KV4_PARTS * (128 + 2) * sizeof(float);
+    const size_t lists = 256 + ((size_t)n_pages / 2 + 1 + S2P_B200_KV4_MAX_LIST) * 8 + (size_t)n_pages * 4;
+    return ((part > lists ? part : lists) + 255) / 256 * 256;
+}
+static inline size_t kv4_work_bytes(int n_pages, int rows, int kv_heads) {
+    return KV4_STATUS_BYTES + kv4_area_bytes(n_pages) + (size_t)rows * (size_t)kv_heads * sizeof(unsigned);
+}
 cudaError_t kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* qkv, const void* q_norm, const void* k_norm,
                        float eps, float rope_base, void* q, cudaStream_t st);
 cudaError_t kv4_read(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, void* k, void* v, cudaStream_t st);

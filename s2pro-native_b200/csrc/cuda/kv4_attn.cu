@@ -26,25 +26,41 @@
 
 namespace s2p {
 
-constexpr int KA_WARPS = 8, KA_THREADS = KA_WARPS * 32, KA_RING = 4;
-constexpr int KA_RING_BYTES = KA_WARPS * KA_RING * KV4_BLOCK_BYTES;
+constexpr int KA_WARPS = 8, KA_THREADS = KA_WARPS * 32, KA_PIECE = 4, KA_STAGES = 2; /* blocks that a warp asks for at a time (of one page), and such pieces in its ring */
+constexpr int KA_RING_BYTES = KA_WARPS * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
 constexpr int KA_PASS = 4;                                         /* columns merged at a time */
 constexpr int KA_MERGE_BYTES = KA_WARPS * KA_PASS * 128 * 4;
-constexpr int KA_LEAST = KA_WARPS;                                 /* blocks that make a CTA worth its while */
+constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 4;           /* blocks that make a worker worth its while */
+constexpr int KA_LONG = 20;                                        /* blocks of a warp from which on warps work by themselves */
 
 struct KaBatch { /* in shared memory, [n (+ 1)] */
-    long long* upto; /* blocks of all units before entry b */
+    unsigned* upto;  /* blocks of all units before entry e */
     int* start;      /* its first row */
+    int* first;      /* its first position, or -1 */
+    int* seq;
 };
-static inline size_t ka_batch_bytes(int n) { return ((size_t)(n + 1) * 12 + 15) / 16 * 16; }
+__host__ __device__ static inline size_t ka_batch_bytes(int n) { return (size_t)(n + 1) * 16; }
+__device__ __forceinline__ KaBatch ka_batch(unsigned char* at, int n) {
+    KaBatch s;
+    s.upto = reinterpret_cast<unsigned*>(at);
+    s.start = reinterpret_cast<int*>(s.upto + n + 1);
+    s.first = s.start + n + 1;
+    s.seq = s.first + n + 1;
+    return s;
+}
 
 __device__ __forceinline__ void ka_mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ka_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
+/* the same onto zeros, without registers set to zero first */
+__device__ __forceinline__ void ka_mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void ka_mma8_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t ka_transpose(uint32_t v) {
     uint32_t r;
@@ -71,7 +87,7 @@ __device__ __forceinline__ uint32_t ka_word(const uint4& v, int i) { return i ==
 template <int NT> struct KaQuery {
     uint32_t b[NT][4][2][2]; /* [column tile][group][half of the group][register] */
     uint32_t sum[NT];        /* sums of q per group, high and low part */
-    float factor[NT][2];     /* of the lane's two score columns: to base-2 logits */
+    float factor[NT][2];     /* of the lane's two score columns: from scores over 2^24 to base-2 logits */
 };
 template <int NT>
 __device__ __forceinline__ void ka_load_query(KaQuery<NT>& z, const __nv_bfloat16* q, size_t row_stride, int group, int columns, int lane) {
@@ -123,7 +139,7 @@ __device__ __forceinline__ void ka_load_query(KaQuery<NT>& z, const __nv_bfloat1
             hi -= __half2float(__float2half_rn(hi));
         }
         z.sum[nt] = ka_half2(lo, hi);
-        const float f = down * (1.4426950408889634f * 0.08838834764831845f); /* log2(e) / sqrt(128) */
+        const float f = down * (16777216.0f * 1.4426950408889634f * 0.08838834764831845f); /* 2^24 log2(e) / sqrt(128) */
         z.factor[nt][0] = __shfl_sync(S2P_FULL_MASK, f, 8 * t);
         z.factor[nt][1] = __shfl_sync(S2P_FULL_MASK, f, 8 * t + 4);
     }
@@ -131,8 +147,8 @@ __device__ __forceinline__ void ka_load_query(KaQuery<NT>& z, const __nv_bfloat1
 
 template <int NT> struct KaState {
     float o[NT][8][4]; /* [column tile][channel tile 2 j + h]: rows 4 g + 2 h (16 times 2^-24 that of the second) and + 1 of group j */
-    float om[NT][4];   /* rows g < 4: sum of p m of group g */
-    float max[NT][2], sum[NT][2];
+    float om[NT][4];   /* [0], [1], in lanes with g < 4: sum of p m of group g; [2], [3]: sum of p */
+    float max[NT][2];
 };
 template <int NT> __device__ __forceinline__ void ka_clear(KaState<NT>& z) {
 #pragma unroll
@@ -144,75 +160,90 @@ template <int NT> __device__ __forceinline__ void ka_clear(KaState<NT>& z) {
 #pragma unroll
         for (int r = 0; r < 4; r++) z.om[nt][r] = 0.0f;
         z.max[nt][0] = z.max[nt][1] = -INFINITY;
-        z.sum[nt][0] = z.sum[nt][1] = 0.0f;
     }
 }
 
-/* One block of 16 positions from shared memory.  `left[..]`: positions of the block that each of the lane's columns sees. */
-template <int NT, bool MASKED>
-__device__ __forceinline__ void ka_block(KaState<NT>& z, const KaQuery<NT>& q, const unsigned char* blk, const int (&left)[NT][2], int lane) {
+/* Two blocks of 16 positions from shared memory: their instructions interleave.  Where `masked`, left(column tile, 0 or 1) says how many of the 32
+ * positions the lane's first or second column of the tile sees.  (There is one copy of this code, for the instruction cache: one token at a
+ * short context runs it once, and a second copy for whole blocks cost more there than the test does.) */
+template <int NT, class Left>
+__device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, const unsigned char* const (&blk)[2], bool masked, Left left, int lane) {
+    constexpr int NB = 2;
     const int g = lane >> 2, t = lane & 3;
-    const uint4 k0 = *reinterpret_cast<const uint4*>(blk + lane * 16), k1 = *reinterpret_cast<const uint4*>(blk + 512 + lane * 16);
-    const uint2 sk0 = *reinterpret_cast<const uint2*>(blk + KV4_PARAMS_K + g * 16), sk1 = *reinterpret_cast<const uint2*>(blk + KV4_PARAMS_K + 128 + g * 16);
-    const uint32_t mk0 = *reinterpret_cast<const uint32_t*>(blk + KV4_PARAMS_K + 8 + g * 16 + (t & 1) * 4),
-                   mk1 = *reinterpret_cast<const uint32_t*>(blk + KV4_PARAMS_K + 136 + g * 16 + (t & 1) * 4);
-    float score[NT][4];
+    float score[NB][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int n = 0; n < NB; n++) {
+        const uint4 k0 = *reinterpret_cast<const uint4*>(blk[n] + lane * 16), k1 = *reinterpret_cast<const uint4*>(blk[n] + 512 + lane * 16);
+        const uint2 sk0 = *reinterpret_cast<const uint2*>(blk[n] + KV4_PARAMS_K + g * 16), sk1 = *reinterpret_cast<const uint2*>(blk[n] + KV4_PARAMS_K + 128 + g * 16);
+        const uint32_t mk0 = *reinterpret_cast<const uint32_t*>(blk[n] + KV4_PARAMS_K + 8 + g * 16 + (t & 1) * 4),
+                       mk1 = *reinterpret_cast<const uint32_t*>(blk[n] + KV4_PARAMS_K + 136 + g * 16 + (t & 1) * 4);
 #pragma unroll
-        for (int r = 0; r < 4; r++) score[nt][r] = 0.0f;
+        for (int j = 0; j < 4; j++) {
+            float part[NT][4];
+            uint32_t w0 = ka_word(k0, j), w1 = ka_word(k1, j);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        float part[NT][4];
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    if (h == 0) ka_mma16_first(part[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, q.b[nt][j][h][0], q.b[nt][j][h][1]);
+                    else ka_mma16(part[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, q.b[nt][j][h][0], q.b[nt][j][h][1]);
+                w0 >>= 8;
+                w1 >>= 8;
+            }
+            const float2 a = ka_halves(j < 2 ? sk0.x : sk0.y), b = ka_halves(j < 2 ? sk1.x : sk1.y);
+            const float s0 = (j & 1) ? a.y : a.x, s1 = (j & 1) ? b.y : b.x;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) score[n][nt][r] = j ? fmaf(part[nt][r], r < 2 ? s0 : s1, score[n][nt][r]) : part[nt][r] * (r < 2 ? s0 : s1);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float mk[4];
+            ka_mma8_first(mk, mk0, mk1, q.sum[nt]);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                score[n][nt][r] = fmaf(mk[r], 5.9604645e-8f, score[n][nt][r]); /* 2^-24, like the codes */
+            }
+        }
+    }
+    if (masked) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) part[nt][r] = 0.0f;
-        uint32_t w0 = ka_word(k0, j), w1 = ka_word(k1, j);
+            for (int c = 0; c < 2; c++) {
+                const int see = left(nt, c) - g;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                ka_mma16(part[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, q.b[nt][j][h][0], q.b[nt][j][h][1]);
-            w0 >>= 8;
-            w1 >>= 8;
-        }
-        const float2 a = ka_halves(j < 2 ? sk0.x : sk0.y), b = ka_halves(j < 2 ? sk1.x : sk1.y);
-        const float s0 = (j & 1) ? a.y : a.x, s1 = (j & 1) ? b.y : b.x;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            score[nt][0] = fmaf(part[nt][0], s0, score[nt][0]);
-            score[nt][1] = fmaf(part[nt][1], s0, score[nt][1]);
-            score[nt][2] = fmaf(part[nt][2], s1, score[nt][2]);
-            score[nt][3] = fmaf(part[nt][3], s1, score[nt][3]);
-        }
+                for (int n = 0; n < NB; n++) {
+                    if (16 * n >= see) score[n][nt][c] = -INFINITY;
+                    if (16 * n + 8 >= see) score[n][nt][c + 2] = -INFINITY;
+                }
+            }
     }
-    uint32_t p[NT][2];
     bool over = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        float mk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        ka_mma8(mk, mk0, mk1, q.sum[nt]);
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            score[nt][r] = fmaf(score[nt][r], 16777216.0f, mk[r]) * q.factor[nt][r & 1];
-            if (MASKED && g + 8 * (r >> 1) >= left[nt][r & 1]) score[nt][r] = -INFINITY;
-            over |= score[nt][r] > z.max[nt][r & 1] + 2.0f;
+        for (int c = 0; c < 2; c++) {
+            float top = fmaxf(score[0][nt][c], score[0][nt][c + 2]);
+#pragma unroll
+            for (int n = 1; n < NB; n++) top = fmaxf(top, fmaxf(score[n][nt][c], score[n][nt][c + 2]));
+            over |= top * q.factor[nt][c] > z.max[nt][c] + 2.0f;
         }
-    }
     if (__any_sync(S2P_FULL_MASK, over)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                float top = fmaxf(score[nt][c], score[nt][c + 2]);
+                float top = fmaxf(score[0][nt][c], score[0][nt][c + 2]);
+#pragma unroll
+                for (int n = 1; n < NB; n++) top = fmaxf(top, fmaxf(score[n][nt][c], score[n][nt][c + 2]));
                 top = fmaxf(top, __shfl_xor_sync(S2P_FULL_MASK, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(S2P_FULL_MASK, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(S2P_FULL_MASK, top, 16));
-                top = fmaxf(top, z.max[nt][c]);
+                top = fmaxf(top * q.factor[nt][c], z.max[nt][c]);
                 const float shrink = top == -INFINITY ? 1.0f : ka_exp2(z.max[nt][c] - top);
                 z.max[nt][c] = top;
-                z.sum[nt][c] *= shrink;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     z.o[nt][i][c] *= shrink;
@@ -222,138 +253,235 @@ __device__ __forceinline__ void ka_block(KaState<NT>& z, const KaQuery<NT>& q, c
                 z.om[nt][c + 2] *= shrink;
             }
     }
+    float base2[NT][2]; /* of columns that have seen nothing yet: a finite one */
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        float e[4];
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const float top = z.max[nt][r & 1];
-            e[r] = ka_exp2(score[nt][r] - (MASKED && top == -INFINITY ? 0.0f : top));
-        }
-        z.sum[nt][0] += e[0] + e[2];
-        z.sum[nt][1] += e[1] + e[3];
-        p[nt][0] = ka_transpose(ka_half2(e[0], e[1]));
-        p[nt][1] = ka_transpose(ka_half2(e[2], e[3]));
-    }
-
-    const uint4 v0 = *reinterpret_cast<const uint4*>(blk + 1024 + lane * 16), v1 = *reinterpret_cast<const uint4*>(blk + 1536 + lane * 16);
-    const uint4 sv0 = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + t * 16), sv1 = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 64 + t * 16);
-    uint32_t mv0 = *reinterpret_cast<const uint32_t*>(blk + KV4_PARAMS_V + 128 + t * 16 + (g & 3) * 4),
-             mv1 = *reinterpret_cast<const uint32_t*>(blk + KV4_PARAMS_V + 192 + t * 16 + (g & 3) * 4);
-    if (g >= 4) mv0 = mv1 = 0;
+        for (int c = 0; c < 2; c++) base2[nt][c] = z.max[nt][c] == -INFINITY ? 0.0f : z.max[nt][c];
+    uint32_t p[NB][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) ka_mma16(z.om[nt], mv0, 0, mv1, 0, p[nt][0], p[nt][1]);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        uint32_t w0 = j < 2 ? prmt(v0.x, v0.z, (j & 1) ? 0x7632 : 0x5410) : prmt(v0.y, v0.w, (j & 1) ? 0x7632 : 0x5410);
-        uint32_t w1 = j < 2 ? prmt(v1.x, v1.z, (j & 1) ? 0x7632 : 0x5410) : prmt(v1.y, v1.w, (j & 1) ? 0x7632 : 0x5410);
-        uint32_t b0[NT], b1[NT];
+    for (int n = 0; n < NB; n++)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            b0[nt] = ka_mul2(p[nt][0], ka_word(sv0, j));
-            b1[nt] = ka_mul2(p[nt][1], ka_word(sv1, j));
+            float e[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                e[r] = ka_exp2(fmaf(score[n][nt][r], q.factor[nt][r & 1], -base2[nt][r & 1]));
+            }
+            p[n][nt][0] = ka_transpose(ka_half2(e[0], e[1]));
+            p[n][nt][1] = ka_transpose(ka_half2(e[2], e[3]));
         }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+    for (int n = 0; n < NB; n++) {
+        const uint4 v0 = *reinterpret_cast<const uint4*>(blk[n] + 1024 + lane * 16), v1 = *reinterpret_cast<const uint4*>(blk[n] + 1536 + lane * 16);
+        const uint4 sv0 = *reinterpret_cast<const uint4*>(blk[n] + KV4_PARAMS_V + t * 16), sv1 = *reinterpret_cast<const uint4*>(blk[n] + KV4_PARAMS_V + 64 + t * 16);
+        const uint32_t mv0 = *reinterpret_cast<const uint32_t*>(blk[n] + KV4_PARAMS_V + 128 + t * 16 + (g & 3) * 4),
+                       mv1 = *reinterpret_cast<const uint32_t*>(blk[n] + KV4_PARAMS_V + 192 + t * 16 + (g & 3) * 4);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                ka_mma16(z.o[nt][2 * j + h], w0 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x000F000Fu, w1 & 0x00F000F0u, b0[nt], b1[nt]);
-            w0 >>= 8;
-            w1 >>= 8;
+        for (int nt = 0; nt < NT; nt++) ka_mma16(z.om[nt], mv0, 0x3C003C00u, mv1, 0x3C003C00u, p[n][nt][0], p[n][nt][1]); /* the lower rows: ones */
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t w0 = j < 2 ? prmt(v0.x, v0.z, (j & 1) ? 0x7632 : 0x5410) : prmt(v0.y, v0.w, (j & 1) ? 0x7632 : 0x5410);
+            uint32_t w1 = j < 2 ? prmt(v1.x, v1.z, (j & 1) ? 0x7632 : 0x5410) : prmt(v1.y, v1.w, (j & 1) ? 0x7632 : 0x5410);
+            uint32_t b0[NT], b1[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                b0[nt] = ka_mul2(p[n][nt][0], ka_word(sv0, j));
+                b1[nt] = ka_mul2(p[n][nt][1], ka_word(sv1, j));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    ka_mma16(z.o[nt][2 * j + h], w0 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x000F000Fu, w1 & 0x00F000F0u, b0[nt], b1[nt]);
+                w0 >>= 8;
+                w1 >>= 8;
+            }
         }
     }
 }
 
+/* Partial results.  CTAs: slot w for part w.  Warps: slot 2 w + 1 where worker w begins a unit that others end, 2 w where it goes on with one. */
 struct KaParts {
-    float *max, *sum, *o; /* [slot][column](, [128]) */
-    unsigned* arrived;    /* [unit] */
+    float *max, *sum, *o; /* [slot][8 NT columns](, [128]) */
+    unsigned* arrived;    /* [row][kv head] of a unit's first row */
 };
 
+/* What the workers from, from + step, ... up to `last` left of a unit (per: slots of a worker; starts: the warp that begins it), for columns base .. base + 3: running
+ * maximum, sum, and channels 4 lane .. 4 lane + 3 of the weighted values.  Sixteen loads are under way at a time. */
+template <int COLS>
+__device__ __forceinline__ void ka_gather(const KaParts& parts, int per, int starts, int from, int step, int last, int base, int columns, int lane, float (&top)[KA_PASS],
+                                          float (&sum)[KA_PASS], float4 (&acc)[KA_PASS]) {
+#pragma unroll
+    for (int k = 0; k < KA_PASS; k++) {
+        top[k] = -INFINITY;
+        sum[k] = 0.0f;
+        acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (int w0 = from; w0 <= last; w0 += 4 * step) {
+        float4 v[4][KA_PASS];
+        float m[4][KA_PASS], l[4][KA_PASS];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int w = w0 + i * step;
+            const size_t at = (size_t)(per * w + (w == starts)) * COLS + base;
+#pragma unroll
+            for (int k = 0; k < KA_PASS; k++) {
+                const bool there = w <= last && base + k < columns;
+                m[i][k] = there ? __ldcg(parts.max + at + k) : -INFINITY;
+                l[i][k] = there ? __ldcg(parts.sum + at + k) : 0.0f;
+                v[i][k] = there ? __ldcg(reinterpret_cast<const float4*>(parts.o + (at + k) * 128) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KA_PASS; k++) {
+            const float now = fmaxf(fmaxf(fmaxf(m[0][k], m[1][k]), fmaxf(m[2][k], m[3][k])), top[k]);
+            const float base2 = now == -INFINITY ? 0.0f : now, keep = ka_exp2(top[k] - base2);
+            sum[k] *= keep;
+            acc[k].x *= keep; acc[k].y *= keep; acc[k].z *= keep; acc[k].w *= keep;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float scale = ka_exp2(m[i][k] - base2);
+                sum[k] = fmaf(l[i][k], scale, sum[k]);
+                acc[k].x = fmaf(v[i][k].x, scale, acc[k].x);
+                acc[k].y = fmaf(v[i][k].y, scale, acc[k].y);
+                acc[k].z = fmaf(v[i][k].z, scale, acc[k].z);
+                acc[k].w = fmaf(v[i][k].w, scale, acc[k].w);
+            }
+            top[k] = now;
+        }
+    }
+}
+
+__device__ __forceinline__ void ka_store(__nv_bfloat16* to, float4 v, float sum) {
+    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * r, v.y * r), hi = __floats2bfloat162_rn(v.z * r, v.w * r);
+    *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
+/* One more worker has left its part of a unit that `others` more share; true for the last of them.  By one thread, behind a barrier of
+ * those that wrote; the others read behind a barrier.  The counter is back at zero before anybody can need it again. */
+__device__ __forceinline__ bool ka_arrive(unsigned* counter, int others) {
+    unsigned old;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    if (old != (unsigned)others) return false;
+    *counter = 0;
+    return true;
+}
+
 template <int NT>
-__global__ void __launch_bounds__(KA_THREADS, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(KA_THREADS, 1)
 k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out, KaParts parts) {
+    constexpr int COLS = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float sh_max[KA_WARPS][8 * NT], sh_sum[KA_WARPS][8 * NT];
-    __shared__ long long sh_scan_ll[KA_WARPS];
-    __shared__ int sh_scan[KA_WARPS], sh_last;
+    __shared__ float sh_max[KA_WARPS][COLS], sh_sum[KA_WARPS][COLS];
+    __shared__ unsigned sh_scan[KA_WARPS];
+    __shared__ int sh_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    unsigned char* ring = smem + warp * KA_RING * KV4_BLOCK_BYTES;
+    unsigned char* ring = smem + warp * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
     float* merge = reinterpret_cast<float*>(smem + KA_RING_BYTES);
-    KaBatch batch;
-    batch.upto = reinterpret_cast<long long*>(smem + KA_RING_BYTES + KA_MERGE_BYTES);
-    batch.start = reinterpret_cast<int*>(batch.upto + b.n + 1);
-    const int group = cache.q_heads / cache.kv_heads, rows_per = max(1, 8 * NT / group);
+    const KaBatch batch = ka_batch(smem + KA_RING_BYTES + KA_MERGE_BYTES, b.n);
+    const int group = cache.q_heads / cache.kv_heads, rows_per = max(1, COLS / group);
     const int capacity = cache.stride * S2P_B200_KV4_PAGE;
 
     grid_wait();
     grid_release();
     /* Rows and blocks of every entry.  Starts are made ascending and kept inside the activations, whatever row0 holds. */
-    const int per = (b.n + KA_THREADS) / KA_THREADS; /* entries a thread looks at, the end of the last among them */
+    auto seen_by = [&](int p0, int row) { /* positions that a row of an entry at p0 sees, its rows counted from 0 */
+        return p0 < 0 ? 0 : (int)min((long long)p0 + row + 1, (long long)capacity);
+    };
+    auto blocks_of = [&](int e) { /* of each of the entry's units */
+        return max(1, (seen_by(batch.first[e], batch.start[e + 1] - batch.start[e] - 1) + 15) / 16);
+    };
+    auto units_of = [&](int e) { return (batch.start[e + 1] - batch.start[e] + rows_per - 1) / rows_per * cache.kv_heads; };
+    const int per = b.n / KA_THREADS + 1; /* entries of a thread, the end of the last among them */
     {
         int top = 0;
-        for (int i = 0; i < per; i++) {
-            const int e = tid * per + i;
-            if (e <= b.n) top = max(top, min(b.row0[e], b.rows));
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
+            const int r = b.row0[e];
+            if (e < b.n) {
+                const int seq = b.seqs[e], p0 = b.pos0[e];
+                batch.seq[e] = seq;
+                batch.first[e] = (unsigned)seq < (unsigned)cache.max_seqs && p0 <= (1 << 30) ? p0 : -1;
+            }
+            top = max(top, min(r, b.rows));
+            batch.start[e] = min(r, b.rows);
         }
-        int incl = top;
+        int before = top;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(S2P_FULL_MASK, incl, off);
-            if (lane >= off) incl = max(incl, o);
+            const int o = __shfl_up_sync(S2P_FULL_MASK, before, off);
+            if (lane >= off) before = max(before, o);
         }
-        if (lane == 31) sh_scan[warp] = incl;
-        int before = __shfl_up_sync(S2P_FULL_MASK, incl, 1);
+        if (lane == 31) sh_scan[warp] = (unsigned)before;
+        before = __shfl_up_sync(S2P_FULL_MASK, before, 1);
         if (lane == 0) before = 0;
         __syncthreads();
-        for (int w = 0; w < warp; w++) before = max(before, sh_scan[w]);
-        for (int i = 0; i < per; i++) {
-            const int e = tid * per + i;
-            if (e <= b.n) batch.start[e] = before = max(before, min(b.row0[e], b.rows));
-        }
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) before = max(before, w < warp ? (int)sh_scan[w] : 0);
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) batch.start[e] = before = max(before, batch.start[e]);
         __syncthreads();
     }
-    auto first_of = [&](int e) { return (unsigned)b.seqs[e] < (unsigned)cache.max_seqs && b.pos0[e] <= (1 << 30) ? b.pos0[e] : -1; };
-    /* positions that the row of an entry at p0 sees, its rows counted from 0 */
-    auto seen_by = [&](int p0, int row) { return p0 < 0 ? 0 : (int)min((long long)p0 + row + 1, (long long)capacity); };
-    auto blocks_of = [&](int e) { /* of each of the entry's units */
-        return max(1, (seen_by(first_of(e), batch.start[e + 1] - batch.start[e] - 1) + 15) / 16);
-    };
-    {
-        long long sum = 0;
-        for (int i = 0; i < per; i++) {
-            const int e = tid * per + i;
-            if (e < b.n) {
-                const int rows = batch.start[e + 1] - batch.start[e];
-                sum += (long long)((rows + rows_per - 1) / rows_per) * cache.kv_heads * blocks_of(e);
-            }
-        }
-        long long incl = sum;
+    /* before[e] and the sum over all entries of what `of` gives for each */
+    auto line_up = [&](auto of) {
+        unsigned sum = 0, all = 0;
+        for (int i = 0, e = tid * per; i < per && e < b.n; i++, e++) sum += of(e);
+        unsigned at = sum;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const long long o = __shfl_up_sync(S2P_FULL_MASK, incl, off);
-            if (lane >= off) incl += o;
+            const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
+            if (lane >= off) at += o;
         }
-        if (lane == 31) sh_scan_ll[warp] = incl;
+        __syncthreads(); /* upto and sh_scan may be read still */
+        if (lane == 31) sh_scan[warp] = at;
+        at -= sum;
         __syncthreads();
-        long long at = incl - sum;
-        for (int w = 0; w < warp; w++) at += sh_scan_ll[w];
-        for (int i = 0; i < per; i++) {
-            const int e = tid * per + i;
-            if (e <= b.n) batch.upto[e] = at;
-            if (e < b.n) {
-                const int rows = batch.start[e + 1] - batch.start[e];
-                at += (long long)((rows + rows_per - 1) / rows_per) * cache.kv_heads * blocks_of(e);
-            }
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) {
+            at += w < warp ? sh_scan[w] : 0;
+            all += sh_scan[w];
+        }
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
+            batch.upto[e] = at;
+            if (e < b.n) at += of(e);
         }
         __syncthreads();
+        return all;
+    };
+    const unsigned total = line_up([&](int e) { return (unsigned)units_of(e) * (unsigned)blocks_of(e); });
+    unsigned units = 0;
+    for (int i = 0, e = tid * per; i < per && e < b.n; i++, e++) units += (unsigned)units_of(e);
+    units = (unsigned)__reduce_add_sync(S2P_FULL_MASK, units);
+    if (lane == 0) sh_scan[warp] = units;
+    __syncthreads();
+    units = 0;
+#pragma unroll
+    for (int w = 0; w < KA_WARPS; w++) units += sh_scan[w];
+    if (!total) return;
+
+    /* Few units on short sequences: each is cut into parts, a CTA to a part, its warps a stretch of it each.  Otherwise warps work by
+     * themselves (no barriers, but a partial for every warp) on equal stretches of the line of all units' blocks. */
+    const bool by_warp = total >= gridDim.x * KA_WARPS * KA_LONG || 2 * units > gridDim.x;
+    unsigned begin, end, share = 1, more = 0, longest = 1;
+    if (by_warp) {
+        const unsigned workers = min(gridDim.x * KA_WARPS, (total + KA_LEAST_WARP - 1) / KA_LEAST_WARP), worker = warp * gridDim.x + blockIdx.x;
+        if (worker >= workers) return;
+        /* worker w has `share` blocks of the line, the first `more` workers one more */
+        share = total / workers;
+        more = total - share * workers;
+        begin = share * worker + min(worker, more);
+        end = begin + share + (worker < more);
+    } else {
+        longest = max((unsigned)KA_LEAST_CTA, (total + gridDim.x - units - 1) / (gridDim.x - units)); /* so there are at most gridDim.x parts */
+        const unsigned parts_all = line_up([&](int e) { return (unsigned)units_of(e) * ((blocks_of(e) + longest - 1) / longest); });
+        begin = blockIdx.x;
+        end = begin + 1;
+        if (begin >= parts_all) return;
     }
-    const long long total = batch.upto[b.n];
-    const long long ctas = min((long long)gridDim.x, (total + KA_LEAST - 1) / KA_LEAST);
-    if (blockIdx.x >= ctas) return;
-    const long long begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+    auto worker_of = [&](unsigned x) { return x < (share + 1) * more ? x / (share + 1) : more + (x - (share + 1) * more) / share; };
 
     int e = 0;
-    { /* the last entry that begins at or before `begin` and has blocks */
+    { /* the last entry that begins at or before `begin` */
         int lo = 0, hi = b.n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -361,190 +489,228 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out,
         }
         e = lo;
     }
-    for (long long cur = begin; cur < end;) {
-        while (batch.upto[e + 1] <= cur) e++;
+    for (unsigned cur = begin; cur < end;) {
+        while (batch.upto[e + 1] <= cur) e++; /* entries without rows */
         const int blocks = blocks_of(e), rows = batch.start[e + 1] - batch.start[e];
-        const long long inside = cur - batch.upto[e];
-        const int unit = (int)(inside / blocks), x0 = (int)(inside % blocks);
-        const int x1 = (int)min((long long)blocks, x0 + (end - cur));
-        const int chunk = unit / cache.kv_heads, head = unit % cache.kv_heads;
+        const unsigned inside = cur - batch.upto[e];
+        unsigned unit;
+        int x0, x1, w0, w1; /* the blocks of this stretch, and the workers of the unit */
+        if (by_warp) {
+            unit = inside / (unsigned)blocks;
+            x0 = (int)(inside - unit * (unsigned)blocks);
+            x1 = x0 + (int)min((unsigned)(blocks - x0), end - cur);
+            w0 = (int)worker_of(cur - (unsigned)x0);
+            w1 = (int)worker_of(cur - (unsigned)x0 + (unsigned)blocks - 1);
+        } else {
+            const int cuts = (int)((blocks + longest - 1) / longest);
+            unit = inside / (unsigned)cuts;
+            const int cut = (int)(inside - unit * (unsigned)cuts), piece = blocks / cuts, rest = blocks - piece * cuts;
+            x0 = piece * cut + min(cut, rest);
+            x1 = x0 + piece + (cut < rest);
+            w0 = (int)cur - cut;
+            w1 = w0 + cuts - 1;
+        }
+        const int chunk = (int)(unit / (unsigned)cache.kv_heads), head = (int)unit - chunk * cache.kv_heads;
         const int r0 = chunk * rows_per, n_rows = min(rows_per, rows - r0), columns = n_rows * group;
-        const int row = batch.start[e] + r0, seq = b.seqs[e], p0 = first_of(e);
+        const int row = batch.start[e] + r0, seq = batch.seq[e], p0 = batch.first[e];
         const int seen = seen_by(p0, r0 + n_rows - 1), least = seen_by(p0, r0); /* by the last row and the first */
         const size_t q_stride = (size_t)cache.q_heads * 128;
 
-        KaQuery<NT> query;
-        ka_load_query<NT>(query, q + (size_t)row * q_stride + (size_t)head * group * 128, q_stride, group, columns, lane);
-        KaState<NT> z;
-        ka_clear(z);
-        int limit[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int col = nt * 8 + 2 * t + c;
-                limit[nt][c] = col < columns ? seen_by(p0, r0 + col / group) : seen;
-            }
-
-        /* this warp's blocks: x0 + warp, + KA_WARPS, ...; lane i keeps the page of the (32 n + i)-th */
-        const int mine = x1 - x0 > warp ? (x1 - x0 - warp + KA_WARPS - 1) / KA_WARPS : 0;
+        /* This warp's blocks, in pieces that end where a page does; lane i keeps the page of the (32 n + i)-th piece. */
+        const int xa = by_warp ? x0 : x0 + (x1 - x0) / KA_WARPS * warp + min(warp, (x1 - x0) % KA_WARPS), xb = by_warp ? x1 : xa + (x1 - x0) / KA_WARPS + (warp < (x1 - x0) % KA_WARPS);
+        const int pieces = xb > xa ? (xb - 1) / KA_PIECE - xa / KA_PIECE + 1 : 0;
         int page_of = -1;
-        unsigned absent = 0; /* ring slots without a block */
+        unsigned absent = 0; /* stages without a page */
         auto fetch = [&](int i) {
-            if (i < mine) {
-                if ((i & 31) == 0) {
-                    const int x = x0 + warp + (i + lane) * KA_WARPS;
-                    page_of = i + lane < mine && x * 16 < seen ? kv4_page(cache, seq, x * 16) : -1;
-                }
-                const int page = __shfl_sync(S2P_FULL_MASK, page_of, i & 31), x = x0 + warp + i * KA_WARPS;
-                const unsigned bit = 1u << (i % KA_RING);
-                if (page >= 0) {
-                    const unsigned char* src = kv4_block(cache, page, head, x * 16) + lane * 16;
-                    const uint32_t dst = smem_u32(ring + (i % KA_RING) * KV4_BLOCK_BYTES) + lane * 16;
+            if (i < pieces) {
+                const int at = xa / KA_PIECE + i;
+                if ((i & 31) == 0) page_of = i + lane < pieces ? kv4_page(cache, seq, (at + lane) * KA_PIECE * 16) : -1;
+                const int page = __shfl_sync(S2P_FULL_MASK, page_of, i & 31);
+                const int from = max(xa, KA_PIECE * at), n = min(min(xb, KA_PIECE * (at + 1)), (seen + 15) / 16) - from; /* (an entry that sees nothing has a block, too) */
+                const unsigned bit = 1u << (i % KA_STAGES);
+                if (page >= 0 && n > 0) {
+                    const unsigned char* src = kv4_block(cache, page, head, from * 16) + lane * 16;
+                    uint32_t dst = smem_u32(ring) + (i % KA_STAGES) * KA_PIECE * KV4_BLOCK_BYTES + lane * 16;
+                    for (int x = 0; x < n; x++, src += KV4_BLOCK_BYTES, dst += KV4_BLOCK_BYTES)
 #pragma unroll
-                    for (int k = 0; k < KV4_BLOCK_BYTES / 512; k++)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 512), "l"(src + k * 512) : "memory");
+                        for (int k = 0; k < KV4_BLOCK_BYTES / 512; k++)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 512), "l"(src + k * 512) : "memory");
                     absent &= ~bit;
                 } else absent |= bit;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int i = 0; i < KA_RING - 1; i++) fetch(i);
-        for (int i = 0; i < mine; i++) {
-            fetch(i + KA_RING - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(KA_RING - 1) : "memory");
+        for (int i = 0; i < KA_STAGES - 1; i++) fetch(i);
+
+        KaQuery<NT> query;
+        ka_load_query<NT>(query, q + (size_t)row * q_stride + (size_t)head * group * 128, q_stride, group, columns, lane);
+        KaState<NT> z;
+        ka_clear(z);
+        for (int i = 0; i < pieces; i++) {
+            fetch(i + KA_STAGES - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(KA_STAGES - 1) : "memory");
             __syncwarp();
-            if (!(absent >> (i % KA_RING) & 1)) {
-                unsigned char* blk = ring + (i % KA_RING) * KV4_BLOCK_BYTES;
-                const int first = (x0 + warp + i * KA_WARPS) * 16;
-                if (first + 16 <= least) {
-                    const int none[NT][2] = {};
-                    ka_block<NT, false>(z, query, blk, none, lane);
-                } else {
-                    if (first + 16 > seen) { /* nobody has written what lies behind the last position: it must not meet a zero weight as NaN */
-                        const int i16 = lane & 15, at = kv4_value_param_at(i16, 0) + (lane >> 4) * 128;
-                        if (first + i16 >= seen)
+            if (!(absent >> (i % KA_STAGES) & 1)) {
+                unsigned char* blk = ring + (i % KA_STAGES) * KA_PIECE * KV4_BLOCK_BYTES;
+                int x = max(xa, KA_PIECE * (xa / KA_PIECE + i));
+                const int to = min(min(xb, KA_PIECE * (xa / KA_PIECE + i + 1)), (seen + 15) / 16), plain = min(to, least / 16); /* blocks that every row sees whole */
+                for (; x < to; x += 2, blk += 2 * KV4_BLOCK_BYTES) {
+                    const int first = x * 16;
+                    if (first + 32 > seen) { /* nobody has written what lies behind the last position: it must not meet a zero weight as NaN */
+                        const int behind = first + lane;
+                        unsigned char* at = blk + (lane >> 4) * KV4_BLOCK_BYTES + kv4_value_param_at(lane & 15, 0);
+                        if (behind >= seen && x + (lane >> 4) < to)
 #pragma unroll
-                            for (int j = 0; j < 4; j++) *reinterpret_cast<uint16_t*>(blk + at + 4 * j) = 0;
+                            for (int j = 0; j < 4; j++) *reinterpret_cast<uint16_t*>(at + 4 * j) = *reinterpret_cast<uint16_t*>(at + 128 + 4 * j) = 0;
                         __syncwarp();
                     }
-                    int left[NT][2];
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        left[nt][0] = limit[nt][0] - first;
-                        left[nt][1] = limit[nt][1] - first;
-                    }
-                    ka_block<NT, true>(z, query, blk, left, lane);
+                    /* an odd last block comes twice, the second time behind everybody's sight */
+                    const unsigned char* const two[2] = {blk, x + 1 < to ? blk + KV4_BLOCK_BYTES : blk};
+                    const int most = x + 1 < to ? 32 : 16;
+                    ka_blocks<NT>(z, query, two, x + 1 >= plain, [&](int nt, int c) {
+                        const int col = nt * 8 + 2 * t + c;
+                        return min(most, (col < columns ? seen_by(p0, r0 + col / group) : seen) - first);
+                    }, lane);
                 }
             }
             __syncwarp();
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-        /* the warps' results together */
+        /* the m term of a group to the lanes that hold its channels */
+        float m_term[NT][2][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                float s = z.sum[nt][c];
-                s += __shfl_xor_sync(S2P_FULL_MASK, s, 4);
-                s += __shfl_xor_sync(S2P_FULL_MASK, s, 8);
-                s += __shfl_xor_sync(S2P_FULL_MASK, s, 16);
-                if (g == 0) {
-                    sh_max[warp][nt * 8 + 2 * t + c] = z.max[nt][c];
-                    sh_sum[warp][nt * 8 + 2 * t + c] = s;
-                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) m_term[nt][c][j] = __shfl_sync(S2P_FULL_MASK, z.om[nt][c], 4 * j + t);
             }
+        auto channels = [&](int nt, int c, int j) { /* 32 j + 4 g .. + 3 of column 8 nt + 2 t + c */
+            const float m = m_term[nt][c][j];
+            return make_float4(fmaf(z.o[nt][2 * j][c], 16777216.0f, m), fmaf(z.o[nt][2 * j][c + 2], 1048576.0f, m), fmaf(z.o[nt][2 * j + 1][c], 16777216.0f, m),
+                               fmaf(z.o[nt][2 * j + 1][c + 2], 1048576.0f, m));
+        };
         const bool whole = x0 == 0 && x1 == blocks;
-        const size_t slot = 2 * (size_t)blockIdx.x + (x0 == 0 ? 1 : 0);
-        const int col = tid >> 6, dim = (tid & 63) * 2;
+        const size_t slot = by_warp ? 2 * (size_t)(warp * gridDim.x + blockIdx.x) + (x0 == 0 ? 1 : 0) : (size_t)cur;
+        unsigned* arrived = parts.arrived + (size_t)row * cache.kv_heads + head;
+        auto out_of = [&](int col) { return out + (size_t)(row + col / group) * q_stride + (size_t)(head * group + col % group) * 128; };
+
+        if (by_warp) {
 #pragma unroll
-        for (int pass = 0; pass < 2 * NT; pass++) {
-            if (pass * KA_PASS >= columns) break;
-            const int nt = pass >> 1;
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                float* to = merge + ((warp * KA_PASS) + 2 * (t & 1) + c) * 128 + 4 * g;
+                for (int c = 0; c < 2; c++) {
+                    const int col = nt * 8 + 2 * t + c;
+                    if (col >= columns) continue;
+                    if (whole) {
+                        __nv_bfloat16* to = out_of(col) + 4 * g;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float m = __shfl_sync(S2P_FULL_MASK, z.om[nt][c], 4 * j + t);
-                    if ((t >> 1) == (pass & 1))
-                        *reinterpret_cast<float4*>(to + 32 * j) =
-                            make_float4(fmaf(z.o[nt][2 * j][c], 16777216.0f, m), fmaf(z.o[nt][2 * j][c + 2], 1048576.0f, m),
-                                        fmaf(z.o[nt][2 * j + 1][c], 16777216.0f, m), fmaf(z.o[nt][2 * j + 1][c + 2], 1048576.0f, m));
-                }
-            }
-            __syncthreads();
-            const int at = pass * KA_PASS + col;
-            if (at < columns) {
-                float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
+                        for (int j = 0; j < 4; j++) ka_store(to + 32 * j, channels(nt, c, j), z.om[nt][2 + c]);
+                    } else {
+                        float* to = parts.o + (slot * COLS + col) * 128 + 4 * g;
 #pragma unroll
-                for (int w = 0; w < KA_WARPS; w++) top = fmaxf(top, sh_max[w][at]);
-#pragma unroll
-                for (int w = 0; w < KA_WARPS; w++) {
-                    const float scale = sh_max[w][at] == -INFINITY && sh_sum[w][at] == 0.0f ? 0.0f : ka_exp2(sh_max[w][at] - (top == -INFINITY ? 0.0f : top));
-                    const float2 v = *reinterpret_cast<const float2*>(merge + (w * KA_PASS + col) * 128 + dim);
-                    sum = fmaf(sh_sum[w][at], scale, sum);
-                    a0 = fmaf(v.x, scale, a0);
-                    a1 = fmaf(v.y, scale, a1);
-                }
-                if (whole) {
-                    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const __nv_bfloat162 y = __floats2bfloat162_rn(a0 * r, a1 * r);
-                    *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(row + at / group) * q_stride + (size_t)(head * group + at % group) * 128 + dim) = y;
-                } else {
-                    if ((tid & 63) == 0) {
-                        parts.max[slot * KV4_PART_COLS + at] = top;
-                        parts.sum[slot * KV4_PART_COLS + at] = sum;
+                        for (int j = 0; j < 4; j++) *reinterpret_cast<float4*>(to + 32 * j) = channels(nt, c, j);
+                        if (g == 0) {
+                            parts.max[slot * COLS + col] = z.max[nt][c];
+                            parts.sum[slot * COLS + col] = z.om[nt][2 + c];
+                        }
                     }
-                    *reinterpret_cast<float2*>(parts.o + (slot * KV4_PART_COLS + at) * 128 + dim) = make_float2(a0, a1);
+                }
+            if (!whole) {
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) last = ka_arrive(arrived, w1 - w0);
+                if (__shfl_sync(S2P_FULL_MASK, last, 0)) {
+                    for (int base = 0; base < columns; base += KA_PASS) {
+                        float top[KA_PASS], sum[KA_PASS];
+                        float4 acc[KA_PASS];
+                        ka_gather<COLS>(parts, 2, w0, w0, 1, w1, base, columns, lane, top, sum, acc);
+#pragma unroll
+                        for (int k = 0; k < KA_PASS; k++)
+                            if (base + k < columns) ka_store(out_of(base + k) + 4 * lane, acc[k], sum[k]);
+                    }
                 }
             }
-            __syncthreads();
-        }
-        if (!whole) {
-            /* CTA of block x of the line: the largest c with total c / ctas <= x */
-            const long long u0 = batch.upto[e] + (long long)unit * blocks, u1 = u0 + blocks - 1;
-            const int c0 = (int)(((u0 + 1) * ctas - 1) / total), c1 = (int)(((u1 + 1) * ctas - 1) / total);
-            if (tid == 0) {
-                /* the row's first column stands for the unit: rows of units are distinct */
-                unsigned* arrived = parts.arrived + (size_t)row * cache.kv_heads + head;
-                __threadfence();
-                const unsigned old = atomicAdd(arrived, 1u);
-                sh_last = old == (unsigned)(c1 - c0);
-                if (sh_last) *arrived = 0;
-                __threadfence();
-            }
-            __syncthreads();
-            if (sh_last) {
-                for (int at = col; at < columns; at += KA_PASS) {
+        } else {
+            /* Four columns at a time through shared memory.  First the warps' own results; then, in the last CTA of a shared unit, what
+             * each warp has gathered of the CTAs' results. */
+            const int col = tid >> 6, dim = (tid & 63) * 2; /* threads 0 .. 255 */
+            auto together = [&](int base, bool to_out) {
+                __syncthreads();
+                const int at = base + col;
+                if (col < KA_PASS && at < columns) {
                     float top = -INFINITY, sum = 0.0f, a0 = 0.0f, a1 = 0.0f;
-                    for (int c = c0; c <= c1; c++) {
-                        const size_t s = 2 * (size_t)c + (total * c / ctas <= u0 ? 1 : 0);
-                        top = fmaxf(top, __ldcg(parts.max + s * KV4_PART_COLS + at));
-                    }
-                    for (int c = c0; c <= c1; c++) {
-                        const size_t s = (2 * (size_t)c + (total * c / ctas <= u0 ? 1 : 0)) * KV4_PART_COLS + at;
-                        const float m = __ldcg(parts.max + s), l = __ldcg(parts.sum + s);
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(parts.o + s * 128 + dim));
-                        const float scale = m == -INFINITY && l == 0.0f ? 0.0f : ka_exp2(m - (top == -INFINITY ? 0.0f : top));
-                        sum = fmaf(l, scale, sum);
+#pragma unroll
+                    for (int w = 0; w < KA_WARPS; w++) top = fmaxf(top, sh_max[w][at]);
+                    const float base2 = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                    for (int w = 0; w < KA_WARPS; w++) {
+                        const float scale = ka_exp2(sh_max[w][at] - base2);
+                        const float2 v = *reinterpret_cast<const float2*>(merge + (w * KA_PASS + col) * 128 + dim);
+                        sum = fmaf(sh_sum[w][at], scale, sum);
                         a0 = fmaf(v.x, scale, a0);
                         a1 = fmaf(v.y, scale, a1);
                     }
-                    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const __nv_bfloat162 y = __floats2bfloat162_rn(a0 * r, a1 * r);
-                    *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(row + at / group) * q_stride + (size_t)(head * group + at % group) * 128 + dim) = y;
+                    if (to_out) {
+                        const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        *reinterpret_cast<__nv_bfloat162*>(out_of(at) + dim) = __floats2bfloat162_rn(a0 * r, a1 * r);
+                    } else {
+                        if ((tid & 63) == 0) {
+                            parts.max[slot * COLS + at] = top;
+                            parts.sum[slot * COLS + at] = sum;
+                        }
+                        *reinterpret_cast<float2*>(parts.o + (slot * COLS + at) * 128 + dim) = make_float2(a0, a1);
+                    }
                 }
+                __syncthreads();
+            };
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+                    if (g == 0) {
+                        sh_max[warp][nt * 8 + 2 * t + c] = z.max[nt][c];
+                        sh_sum[warp][nt * 8 + 2 * t + c] = z.om[nt][2 + c];
+                    }
+#pragma unroll
+            for (int pass = 0; pass < 2 * NT; pass++) {
+                if (pass * KA_PASS >= columns) break;
+                if ((t >> 1) == (pass & 1)) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            *reinterpret_cast<float4*>(merge + (warp * KA_PASS + 2 * (t & 1) + c) * 128 + 32 * j + 4 * g) = channels(pass >> 1, c, j);
+                }
+                together(pass * KA_PASS, whole);
             }
-            __syncthreads();
+            if (!whole) {
+                if (tid == 0) sh_last = ka_arrive(arrived, w1 - w0);
+                __syncthreads();
+                if (sh_last) {
+                    for (int base = 0; base < columns; base += KA_PASS) {
+                        float top[KA_PASS], sum[KA_PASS];
+                        float4 acc[KA_PASS];
+                        ka_gather<COLS>(parts, 1, -1, w0 + warp, KA_WARPS, w1, base, columns, lane, top, sum, acc);
+#pragma unroll
+                        for (int k = 0; k < KA_PASS; k++) {
+                            if (base + k < COLS && lane == 0) {
+                                sh_max[warp][base + k] = top[k];
+                                sh_sum[warp][base + k] = sum[k];
+                            }
+                            *reinterpret_cast<float4*>(merge + (warp * KA_PASS + k) * 128 + 4 * lane) = acc[k];
+                        }
+                        together(base, true);
+                    }
+                }
+                __syncthreads();
+            }
         }
-        cur += x1 - x0;
+        cur += by_warp ? x1 - x0 : 1;
     }
 }
-
-extern "C" size_t kv4_counter_bytes(int rows, int kv_heads) { return ((size_t)rows * (size_t)kv_heads * sizeof(unsigned) + 255) / 256 * 256; }
 
 template <int NT>
 static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* q, void* out, cudaStream_t st) {
@@ -563,14 +729,13 @@ static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
         attr_set[dev] = true;
     }
     KaParts p;
-    unsigned char* at = static_cast<unsigned char*>(c->work) + KV4_STATUS_BYTES;
-    p.arrived = reinterpret_cast<unsigned*>(at);
-    at += kv4_counter_bytes(b->rows, c->kv_heads);
-    p.o = reinterpret_cast<float*>(at);
-    p.max = p.o + (size_t)2 * KV4_MAX_CTAS * KV4_PART_COLS * 128;
-    p.sum = p.max + (size_t)2 * KV4_MAX_CTAS * KV4_PART_COLS;
-    const int grid = sms[dev] * (NT == 1 ? 2 : 1);
-    return launch_after(k_kv4_attn<NT>, dim3((unsigned)(grid < KV4_MAX_CTAS ? grid : KV4_MAX_CTAS)), KA_THREADS, smem, st, kv4_view(*c, layer), kv4_rows(*b),
+    unsigned char* area = static_cast<unsigned char*>(c->work) + KV4_STATUS_BYTES;
+    p.arrived = reinterpret_cast<unsigned*>(area + kv4_area_bytes(c->n_pages));
+    p.o = reinterpret_cast<float*>(area);
+    p.max = p.o + (size_t)KV4_PARTS * 128;
+    p.sum = p.max + KV4_PARTS;
+    const int grid = sms[dev], most = KV4_PARTS / (2 * KA_WARPS * 8 * NT);
+    return launch_after(k_kv4_attn<NT>, dim3((unsigned)(grid < most ? grid : most)), KA_THREADS, smem, st, kv4_view(*c, layer), kv4_rows(*b),
                         static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), p);
 }
 

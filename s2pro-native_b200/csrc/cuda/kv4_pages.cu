@@ -16,14 +16,11 @@ struct Kv4Lists {
     int* renumber;
 };
 static inline Kv4Lists kv4_lists(const s2p_b200_kv4& c) {
-    /* behind the largest counter area that the workspace was sized for: the lists go to its end */
-    unsigned char* end = static_cast<unsigned char*>(c.work) + c.work_bytes / 256 * 256;
-    const size_t moves = ((size_t)c.n_pages / 2 + 1 + S2P_B200_KV4_MAX_LIST) * sizeof(int2), numbers = (size_t)c.n_pages * sizeof(int);
+    unsigned char* at = static_cast<unsigned char*>(c.work) + KV4_STATUS_BYTES;
     Kv4Lists l;
-    unsigned char* at = end - 256 - (moves + 255) / 256 * 256 - (numbers + 255) / 256 * 256;
     l.words = reinterpret_cast<int*>(at);
     l.moves = reinterpret_cast<int2*>(at + 256);
-    l.renumber = reinterpret_cast<int*>(at + 256 + (moves + 255) / 256 * 256);
+    l.renumber = reinterpret_cast<int*>(l.moves + c.n_pages / 2 + 1 + S2P_B200_KV4_MAX_LIST);
     return l;
 }
 

@@ -17,13 +17,8 @@ size_t s2p_b200_kv4_page_bytes(int layers, int kv_heads) {
     return (size_t)layers * (size_t)kv_heads * KV4_HEAD_BYTES;
 }
 
-/* the page operators keep: a pair of pages per move, a new number per page, and a few words */
-static size_t list_bytes(const s2p_b200_kv4* c) { return (size_t)c->n_pages * 12 + 8 * S2P_B200_KV4_MAX_LIST + 4096; }
-
 size_t s2p_b200_kv4_work_bytes(const s2p_b200_kv4* c, int rows) {
-    if (!sizes_served(c) || rows < 0) return 0;
-    const size_t part = (size_t)2 * KV4_MAX_CTAS * KV4_PART_FLOATS * sizeof(float), lists = list_bytes(c);
-    return KV4_STATUS_BYTES + kv4_counter_bytes(rows, c->kv_heads) + (part > lists ? part : lists);
+    return !sizes_served(c) || rows < 0 ? 0 : kv4_work_bytes(c->n_pages, rows, c->kv_heads);
 }
 
 static s2p_status check_cache(const char* what, const s2p_b200_kv4* c, int rows) {
@@ -121,6 +116,10 @@ s2p_status s2p_b200_kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batc
     S2P_TRY(check_layer("kv4_attention", c, b, b && b->rows > 0 ? b->rows : 0, layer));
     if (!b->n || !b->rows) return S2P_OK;
     if (!q || !out || misaligned(q, 16) || misaligned(out, 16)) return S2P_ERR_INVALID;
+    if ((double)b->rows * c->kv_heads * c->table_stride > (double)KV4_MAX_LINE) {
+        fprintf(stderr, "[s2pro] kv4_attention: rows * kv_heads * table_stride is above %d: split the batch\n", KV4_MAX_LINE);
+        return S2P_ERR_INVALID;
+    }
     S2P_CUDA_TRY(kv4_attention(c, b, layer, q, out, stream));
     return S2P_OK;
 }

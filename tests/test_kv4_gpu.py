@@ -174,7 +174,23 @@ def test_long_sequence_is_put_together_the_same_every_time(mine, capi):
         outs.append(out)
     check_attention(cache, b, [(0, 31999, 0, 1), (2, 8998, 1, 2)], q, outs[0])
     assert all(torch.equal(o, outs[0]) for o in outs)
-    assert not bool(cache.work[:256 + 256].any())
+    assert not bool(cache.work[:256].any()) and not bool(cache.work[-64 * 2 * 4:].any())
+
+
+def test_one_workspace_for_calls_of_all_sizes(mine, capi):
+    """Calls with different numbers of rows, page operators between them: each finds the counters at zero."""
+    cache = _kv4.Cache(mine, capi, 60, kv_heads=2, q_heads=8, max_seqs=3, stride=32, rows=300)
+    _kv4.fill(cache, 0, 1300, seed=1)
+    q = queries(300, 8)
+    for i, rows in enumerate((1, 70, 2, 300, 1, 33, 5, 256, 3, 8)):
+        b = cache.batch([0], [rows], [1300 - rows])
+        out = torch.full_like(q, 7.0)
+        cache.attention(b, q, out)
+        check_attention(cache, b, [(0, 1300 - rows, 0, rows)], q, out)
+        if i % 3 == 2:
+            cache.fork([0], [1], [1000])
+            cache.release([1])
+            cache.compact()
 
 
 def test_offsets_beyond_32_bits(mine, capi):
