@@ -90,4 +90,14 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float x[4], __half& s_out
     return codes;
 }
 
+/* One more worker has left its part of a unit that `others` more share; true for the last of them.  By one thread, behind a barrier of
+ * those that wrote; the others read behind a barrier.  The counter is back at zero before anybody can need it again. */
+__device__ __forceinline__ bool kv4_arrive(unsigned* counter, int others) {
+    unsigned old;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    if (old != (unsigned)others) return false;
+    *counter = 0;
+    return true;
+}
+
 }  // namespace s2p

@@ -23,9 +23,12 @@ namespace s2p {
 extern "C" {
 #endif
 
+#define KV4_SLICE_CTAS 160           /* CTAs of a slices' launch; two partials of 256 rows each */
+
 /* Bytes of the area.  The page operators keep a few words, a pair of pages per move and a new number per page. */
 static inline size_t kv4_area_bytes(int n_pages) {
-    const size_t part = (size_t)KV4_PARTS * (128 + 2) * sizeof(float);
+    const size_t tokens = (size_t)KV4_PARTS * (128 + 2) * sizeof(float), slices = (size_t)2 * KV4_SLICE_CTAS * 256 * (128 + 2) * sizeof(float);
+    const size_t part = tokens > slices ? tokens : slices;
     const size_t lists = 256 + ((size_t)n_pages / 2 + 1 + S2P_B200_KV4_MAX_LIST) * 8 + (size_t)n_pages * 4;
     return ((part > lists ? part : lists) + 255) / 256 * 256;
 }
@@ -36,6 +39,9 @@ cudaError_t kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int l
                        float eps, float rope_base, void* q, cudaStream_t st);
 cudaError_t kv4_read(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, void* k, void* v, cudaStream_t st);
 cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* q, void* out, cudaStream_t st);
+/* slices of more than `few` rows, where the batch's chunks fit in shared memory */
+int kv4_slices_serve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b);
+cudaError_t kv4_slices(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, int few, const void* q, void* out, cudaStream_t st);
 cudaError_t kv4_reserve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int32_t* info, cudaStream_t st);
 cudaError_t kv4_fork(const s2p_b200_kv4* c, const int32_t* parents, const int32_t* children, const int32_t* tokens, int n, int32_t* info,
                      cudaStream_t st);

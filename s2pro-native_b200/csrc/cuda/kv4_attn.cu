@@ -21,6 +21,7 @@
  * CTA takes an equal stretch of it, its warps the stretch's blocks in turn through a ring of asynchronous copies of their own; a
  * unit that several CTAs share is put together by the last of them to arrive, in the CTAs' order, so that the result does not
  * depend on timing. */
+#include <limits.h>
 #include "kv4.cuh"
 #include "pipe.cuh"
 
@@ -31,6 +32,7 @@ constexpr int KA_RING_BYTES = KA_WARPS * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
 constexpr int KA_PASS = 4;                                         /* columns merged at a time */
 constexpr int KA_MERGE_BYTES = KA_WARPS * KA_PASS * 128 * 4;
 constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 4;           /* blocks that make a worker worth its while */
+constexpr int KA_FEW = 32;                                         /* (row, head) columns of a kv head that are still single tokens' work */
 constexpr int KA_LONG = 20;                                        /* blocks of a warp from which on warps work by themselves */
 
 struct KaBatch { /* in shared memory, [n (+ 1)] */
@@ -359,19 +361,9 @@ __device__ __forceinline__ void ka_store(__nv_bfloat16* to, float4 v, float sum)
     *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
-/* One more worker has left its part of a unit that `others` more share; true for the last of them.  By one thread, behind a barrier of
- * those that wrote; the others read behind a barrier.  The counter is back at zero before anybody can need it again. */
-__device__ __forceinline__ bool ka_arrive(unsigned* counter, int others) {
-    unsigned old;
-    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
-    if (old != (unsigned)others) return false;
-    *counter = 0;
-    return true;
-}
-
 template <int NT>
 __global__ void __launch_bounds__(KA_THREADS, 1)
-k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out, KaParts parts) {
+k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloat16* out, KaParts parts) {
     constexpr int COLS = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sh_max[KA_WARPS][COLS], sh_sum[KA_WARPS][COLS];
@@ -393,7 +385,10 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out,
     auto blocks_of = [&](int e) { /* of each of the entry's units */
         return max(1, (seen_by(batch.first[e], batch.start[e + 1] - batch.start[e] - 1) + 15) / 16);
     };
-    auto units_of = [&](int e) { return (batch.start[e + 1] - batch.start[e] + rows_per - 1) / rows_per * cache.kv_heads; };
+    auto units_of = [&](int e) { /* entries of more rows than `few` are another kernel's */
+        const int rows = batch.start[e + 1] - batch.start[e];
+        return rows > few ? 0 : (rows + rows_per - 1) / rows_per * cache.kv_heads;
+    };
     const int per = b.n / KA_THREADS + 1; /* entries of a thread, the end of the last among them */
     {
         int top = 0;
@@ -621,7 +616,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out,
             if (!whole) {
                 __syncwarp();
                 int last = 0;
-                if (lane == 0) last = ka_arrive(arrived, w1 - w0);
+                if (lane == 0) last = kv4_arrive(arrived, w1 - w0);
                 if (__shfl_sync(S2P_FULL_MASK, last, 0)) {
                     for (int base = 0; base < columns; base += KA_PASS) {
                         float top[KA_PASS], sum[KA_PASS];
@@ -687,7 +682,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out,
                 together(pass * KA_PASS, whole);
             }
             if (!whole) {
-                if (tid == 0) sh_last = ka_arrive(arrived, w1 - w0);
+                if (tid == 0) sh_last = kv4_arrive(arrived, w1 - w0);
                 __syncthreads();
                 if (sh_last) {
                     for (int base = 0; base < columns; base += KA_PASS) {
@@ -713,7 +708,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, const __nv_bfloat16* q, __nv_bfloat16* out,
 }
 
 template <int NT>
-static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* q, void* out, cudaStream_t st) {
+static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, int few, const void* q, void* out, cudaStream_t st) {
     const size_t smem = KA_RING_BYTES + KA_MERGE_BYTES + ka_batch_bytes(b->n);
     static bool attr_set[64] = {false};
     static int sms[64] = {0};
@@ -735,13 +730,19 @@ static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
     p.max = p.o + (size_t)KV4_PARTS * 128;
     p.sum = p.max + KV4_PARTS;
     const int grid = sms[dev], most = KV4_PARTS / (2 * KA_WARPS * 8 * NT);
-    return launch_after(k_kv4_attn<NT>, dim3((unsigned)(grid < most ? grid : most)), KA_THREADS, smem, st, kv4_view(*c, layer), kv4_rows(*b),
+    return launch_after(k_kv4_attn<NT>, dim3((unsigned)(grid < most ? grid : most)), KA_THREADS, smem, st, kv4_view(*c, layer), kv4_rows(*b), few,
                         static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), p);
 }
 
 extern "C" cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* q, void* out, cudaStream_t st) {
-    const int group = c->q_heads / c->kv_heads, rows = b->max_rows > 1 ? b->max_rows : 1;
-    return rows * group <= 8 ? launch_attn<1>(c, b, layer, q, out, st) : launch_attn<2>(c, b, layer, q, out, st);
+    const int group = c->q_heads / c->kv_heads, most = b->max_rows < b->rows ? b->max_rows : b->rows;
+    int few = INT_MAX;
+    if (most * group > KA_FEW && kv4_slices_serve(c, b)) {
+        few = b->n == 1 ? 0 : KA_FEW / group; /* the rows of an entry are known on the device alone: a batch of several may need both kernels */
+        const cudaError_t e = kv4_slices(c, b, layer, few, q, out, st);
+        if (e != cudaSuccess || !few) return e;
+    }
+    return (few < most ? few : most) * group <= 8 ? launch_attn<1>(c, b, layer, few, q, out, st) : launch_attn<2>(c, b, layer, few, q, out, st);
 }
 
 }  // namespace s2p

@@ -1,0 +1,685 @@
+/* Attention of prompt slices over the paged 4-bit cache, on the 5th-generation tensor cores.
+ *
+ * A unit is one kv head of one sequence with two tiles of 128 query rows each: 128 / G consecutive rows of the slice times the G
+ * query heads of that kv head (32 rows at G = 4).  It walks the sequence page by page:
+ *
+ *   S = Q K^T    [128 x 64], tcgen05.mma, both operands in shared memory, f32 in TMEM
+ *   P = 2^(S f - m), f16, over columns that held S; running maximum m and sum in 32 bits, m renewed where a score passes it by 8
+ *   O += P V     [128 x 128], P from TMEM, V in shared memory, f32 in TMEM
+ *
+ * Roles, coupled by mbarriers only:
+ *   warps 0..3, 4..7   one thread a query row of the first, second tile: the row as f16 into shared memory (times a power of two, so that its
+ *                      largest value is 512..1023: exact), then the softmax with the row's 64 scores in registers, at the end the result
+ *   warps 8..11        turn pages into operands: s c + m in f16 (one rounding, 2^-11), keys as [channel / 8][position] units of 8 channels,
+ *                      values likewise; codes and parameters of the next page are under way while this one is converted; four stages
+ *   warp 12            one thread issues the products.  Each row tile has two places for scores, so the scores of page i + 1 are
+ *                      computed while the softmax of page i runs: it never waits for them.
+ * Both row tiles use the same converted keys and values, which is what two of them are for.  Every operand is in the unswizzled
+ * core-matrix layout (8 rows x 16 bytes); a unit plane has 32 or 16 bytes more than its positions take, so that the converting lanes'
+ * stores fall on different banks.
+ *
+ * Work is cut like that of single tokens: the pages of all units form one line, each CTA takes an equal stretch of it, and
+ * the last CTA of a shared unit adds the parts in order. */
+#include "kv4.cuh"
+#include "pipe.cuh"
+
+namespace s2p {
+
+constexpr int KS_ROWS = 128, KS_TILE = S2P_B200_KV4_PAGE, KS_STAGES = 4, KS_THREADS = 13 * 32, KS_SOFTMAX = 256;
+constexpr int KS_Q_BYTES = 16 * 128 * 16;                                  /* one row tile: [channel / 8][row] units */
+constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
+constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
+constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES);
+constexpr int KS_LEAST = 5;                                                /* pages that make a CTA worth its while */
+static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
+
+struct KsBars {
+    uint64_t k_full[KS_STAGES], k_free[KS_STAGES], v_full[KS_STAGES], v_free[KS_STAGES];
+    uint64_t s_full[2][2], p_full[2][2]; /* [row tile][place] */
+    uint64_t o_done[2], q_full, unit_done, all_done;
+};
+
+struct KsLine { /* in shared memory: the chunks (units of one kv head each) of all entries */
+    unsigned* upto;  /* [chunks + 1] position tiles times kv heads before a chunk */
+    int* first;      /* [entries + 1] chunks before an entry */
+    int* start;      /* [entries + 1] rows before an entry */
+};
+static inline size_t ks_line_bytes(int chunks, int n) { return (size_t)(chunks + 1 + 2 * (n + 1)) * 4; }
+
+struct KsParts {
+    float *max, *sum; /* [slot][256 rows] */
+    float4* o;        /* [slot][channel / 4][256 rows] */
+    unsigned* arrived;
+    int* status;
+};
+
+__device__ __forceinline__ uint64_t ks_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void ks_ld32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ks_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ks_ld16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ks_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+          "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ks_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ks_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ks_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ks_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ks_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void ks_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void ks_softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ float ks_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t ks_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ __half2 ks_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t ks_u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+/* eight codes of a word as s c + m: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7 (those of a byte's upper half come as 16 c) */
+__device__ __forceinline__ uint4 ks_widen(uint32_t w, __half2 s, __half2 m) {
+    const __half2 k1024 = ks_h2(0x64006400u), k16th = ks_h2(0x2C002C00u), k64 = ks_h2(0xD400D400u); /* 1024, 1 / 16, -64 */
+    const uint32_t x = w >> 8;
+    uint4 r;
+    r.x = ks_u(__hfma2(__hsub2(ks_h2((w & 0x000F000Fu) | 0x64006400u), k1024), s, m));
+    r.y = ks_u(__hfma2(__hfma2(ks_h2((w & 0x00F000F0u) | 0x64006400u), k16th, k64), s, m));
+    r.z = ks_u(__hfma2(__hsub2(ks_h2((x & 0x000F000Fu) | 0x64006400u), k1024), s, m));
+    r.w = ks_u(__hfma2(__hfma2(ks_h2((x & 0x00F000F0u) | 0x64006400u), k16th, k64), s, m));
+    return r;
+}
+__device__ __forceinline__ uint32_t ks_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+/* Entries of up to `few` rows are left to the kernel for single tokens.  shift: registers of the row's place in a tile. */
+__global__ void __launch_bounds__(KS_THREADS, 1)
+k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloat16* out, KsParts parts) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ KsBars bars;
+    __shared__ uint32_t sh_tmem;
+    __shared__ unsigned sh_scan[13], sh_last;
+    __shared__ int sh_absent[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = cache.q_heads / cache.kv_heads, tile_rows = KS_ROWS / group, unit_rows = 2 * tile_rows;
+    const int capacity = cache.stride * S2P_B200_KV4_PAGE;
+    unsigned char *sq = smem, *sk = sq + 2 * KS_Q_BYTES, *sv = sk + KS_STAGES * KS_K_BYTES;
+    KsLine line;
+    line.first = reinterpret_cast<int*>(smem + KS_OPERANDS);
+    line.start = line.first + b.n + 1;
+    line.upto = reinterpret_cast<unsigned*>(line.start + b.n + 1);
+    int* status = parts.status;
+
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < KS_STAGES; i++) {
+            mbar_init(&bars.k_full[i], 4);
+            mbar_init(&bars.k_free[i], 1);
+            mbar_init(&bars.v_full[i], 4);
+            mbar_init(&bars.v_free[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            for (int j = 0; j < 2; j++) {
+                mbar_init(&bars.s_full[i][j], 1);
+                mbar_init(&bars.p_full[i][j], 4);
+            }
+            mbar_init(&bars.o_done[i], 1);
+        }
+        mbar_init(&bars.q_full, 8);
+        mbar_init(&bars.unit_done, 1);
+        mbar_init(&bars.all_done, 1);
+        mbar_init_fence();
+    }
+    grid_wait();
+    grid_release();
+    ks_before_sync();
+
+    /* ---- the line of work ---- */
+    auto block_scan = [&](unsigned v, unsigned& all) { /* sum over the threads before this one, and over all */
+        unsigned at = v;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
+            if (lane >= off) at += o;
+        }
+        __syncthreads();
+        if (lane == 31) sh_scan[warp] = at;
+        at -= v;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < 13; w++) {
+            at += w < warp ? sh_scan[w] : 0;
+            all += sh_scan[w];
+        }
+        return at;
+    };
+    const int per = b.n / KS_THREADS + 1;
+    {
+        int top = 0; /* starts made ascending and kept inside the activations, whatever row0 holds */
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) top = max(top, line.start[e] = min(b.row0[e], b.rows));
+        int before = top;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(S2P_FULL_MASK, before, off);
+            if (lane >= off) before = max(before, o);
+        }
+        if (lane == 31) sh_scan[warp] = (unsigned)before;
+        before = __shfl_up_sync(S2P_FULL_MASK, before, 1);
+        if (lane == 0) before = 0;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 13; w++) before = max(before, w < warp ? (int)sh_scan[w] : 0);
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) line.start[e] = before = max(before, line.start[e]);
+        __syncthreads();
+    }
+    ks_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh_tmem);
+    auto rows_of = [&](int e) { return line.start[e + 1] - line.start[e]; };
+    auto chunks_of = [&](int e) { return rows_of(e) > few ? (rows_of(e) + unit_rows - 1) / unit_rows : 0; };
+    auto first_of = [&](int e) { return (unsigned)b.seqs[e] < (unsigned)cache.max_seqs && b.pos0[e] <= (1 << 30) ? b.pos0[e] : -1; };
+    auto seen_by = [&](int p0, int row) { return p0 < 0 ? 0 : (int)min((long long)p0 + row + 1, (long long)capacity); };
+    unsigned chunks, total;
+    {
+        unsigned sum = 0;
+        for (int i = 0, e = tid * per; i < per && e < b.n; i++, e++) sum += (unsigned)chunks_of(e);
+        unsigned at = block_scan(sum, chunks);
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
+            line.first[e] = (int)at;
+            if (e < b.n) at += (unsigned)chunks_of(e);
+        }
+        __syncthreads();
+    }
+    auto entry_of = [&](int chunk) { /* the entry whose chunk it is */
+        int lo = 0, hi = b.n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (line.first[mid] <= chunk) lo = mid; else hi = mid;
+        }
+        return lo;
+    };
+    auto tiles_of = [&](int e, int chunk) { /* position tiles of a chunk's unit */
+        const int last = min(rows_of(e), (chunk - line.first[e] + 1) * unit_rows) - 1;
+        return max(1, (seen_by(first_of(e), last) + KS_TILE - 1) / KS_TILE);
+    };
+    {
+        const int each = (int)chunks / KS_THREADS + 1;
+        unsigned sum = 0;
+        for (int i = 0, c = tid * each; i < each && c < (int)chunks; i++, c++) {
+            const unsigned t = (unsigned)tiles_of(entry_of(c), c) * (unsigned)cache.kv_heads;
+            line.upto[c] = t;
+            sum += t;
+        }
+        unsigned at = block_scan(sum, total);
+        for (int i = 0, c = tid * each; i < each && c <= (int)chunks; i++, c++) {
+            const unsigned t = c < (int)chunks ? line.upto[c] : 0;
+            line.upto[c] = at;
+            at += t;
+        }
+        __syncthreads();
+    }
+    const unsigned workers = min(gridDim.x, (total + KS_LEAST - 1) / KS_LEAST);
+    const unsigned share = workers ? total / workers : 1, more = workers ? total - share * workers : 0, worker = blockIdx.x;
+    const unsigned begin = worker < workers ? share * worker + min(worker, more) : 0, end = worker < workers ? begin + share + (worker < more) : 0;
+    auto worker_of = [&](unsigned x) { return x < (share + 1) * more ? x / (share + 1) : more + (x - (share + 1) * more) / share; };
+
+    struct Segment {
+        int e, head, row0, n_rows, seq, p0, seen, t0, t1, tiles, r0;
+        unsigned u0;
+    };
+    int chunk_at = 0;
+    if (begin < end) {
+        int lo = 0, hi = (int)chunks;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (line.upto[mid] <= begin) lo = mid; else hi = mid;
+        }
+        chunk_at = lo;
+    }
+    auto segment = [&](unsigned cur, int& chunk) {
+        Segment s;
+        while (line.upto[chunk + 1] <= cur) chunk++;
+        s.e = entry_of(chunk);
+        s.tiles = tiles_of(s.e, chunk);
+        const unsigned inside = cur - line.upto[chunk];
+        s.head = (int)(inside / (unsigned)s.tiles);
+        s.t0 = (int)(inside - (unsigned)s.head * (unsigned)s.tiles);
+        s.t1 = s.t0 + (int)min((unsigned)(s.tiles - s.t0), end - cur);
+        s.u0 = cur - (unsigned)s.t0;
+        s.r0 = (chunk - line.first[s.e]) * unit_rows;
+        s.n_rows = min(unit_rows, rows_of(s.e) - s.r0);
+        s.row0 = line.start[s.e] + s.r0;
+        s.seq = b.seqs[s.e];
+        s.p0 = first_of(s.e);
+        s.seen = seen_by(s.p0, s.r0 + s.n_rows - 1);
+        return s;
+    };
+
+    if (warp < 8) {
+        /* ================= softmax ================= */
+        const int x = warp >> 2, r = tid & 127; /* row tile, row */
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_o = tmem + (uint32_t)(x * 128) + lanes, t_s = tmem + 256u + (uint32_t)(x * 128) + lanes;
+        unsigned n_s = 0, segments = 0; /* pages of this row tile so far */
+        bool ok = true;
+        int chunk = chunk_at;
+        unsigned it = 0; /* position tiles of the CTA so far */
+        for (unsigned cur = begin; cur < end && ok;) {
+            const Segment s = segment(cur, chunk);
+            const int my_row = x * tile_rows + r / group, my_head = s.head * group + r % group;
+            const bool live = r < tile_rows * group && my_row < s.n_rows, active = x * tile_rows < s.n_rows;
+            const size_t at = ((size_t)(s.row0 + my_row) * cache.q_heads + my_head) * 128;
+            float f = 0.0f;
+            {
+                uint4 raw[16];
+#pragma unroll
+                for (int u = 0; u < 16; u++) raw[u] = live ? reinterpret_cast<const uint4*>(q + at)[u] : make_uint4(0, 0, 0, 0);
+                float big = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 16; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) big = fmaxf(big, fmaxf(fabsf(bf_lo(ks_word(raw[u], i))), fabsf(bf_hi(ks_word(raw[u], i)))));
+                const int e = big > 0.0f ? min(136 - (int)(__float_as_uint(big) >> 23), 120) : 0; /* 2^9 <= big 2^e < 2^10 */
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                f = __uint_as_float((uint32_t)(127 - e) << 23) * (1.4426950408889634f * 0.08838834764831845f); /* to base-2 logits: log2(e) / sqrt(128) */
+#pragma unroll
+                for (int u = 0; u < 16; u++) { /* channels 0, 4, 1, 5, 2, 6, 3, 7 of the unit, as ks_widen puts them */
+                    const uint4 w = raw[u];
+                    uint4 h;
+                    h.x = ks_half2(bf_lo(w.x) * up, bf_lo(w.z) * up);
+                    h.y = ks_half2(bf_hi(w.x) * up, bf_hi(w.z) * up);
+                    h.z = ks_half2(bf_lo(w.y) * up, bf_lo(w.w) * up);
+                    h.w = ks_half2(bf_hi(w.y) * up, bf_hi(w.w) * up);
+                    *reinterpret_cast<uint4*>(sq + x * KS_Q_BYTES + (u * 128 + r) * 16) = h;
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.q_full);
+
+            const int limit = live ? seen_by(s.p0, s.r0 + my_row) : s.seen;
+            float top = -INFINITY, sum = 0.0f;
+            if (active)
+                for (int i = s.t0; i < s.t1; i++, n_s++) {
+                    const unsigned place = n_s & 1;
+                    ok = mbar_wait_warp(&bars.s_full[x][place], (n_s >> 1) & 1, status);
+                    if (!ok) break;
+                    ks_after_sync();
+                    uint32_t v[2][32];
+                    ks_ld32(t_s + 64 * place, v[0]);
+                    ks_ld32(t_s + 64 * place + 32, v[1]);
+                    const int left = *reinterpret_cast<volatile int*>(&sh_absent[(it + (unsigned)(i - s.t0)) & 7]) ? 0 : limit - i * KS_TILE;
+                    ks_ld_wait();
+                    if (__any_sync(S2P_FULL_MASK, left < KS_TILE)) {
+#pragma unroll
+                        for (int k = 0; k < 64; k++)
+                            if (k >= left) v[k >> 5][k & 31] = 0xFF800000u;
+                    }
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 64; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k >> 5][k & 31]));
+                    const float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+                    if (__any_sync(S2P_FULL_MASK, most > top + 8.0f)) {
+                        const float now = fmaxf(most, top), shrink = now == -INFINITY ? 1.0f : ks_exp2(top - now);
+                        top = now;
+                        sum *= shrink;
+                        if (i > s.t0) { /* behind the product of the page before; the one before that was waited for in front of these scores */
+                            ok = mbar_wait_warp(&bars.o_done[x], (n_s - 1) & 1, status);
+                            if (!ok) break;
+                            ks_after_sync();
+#pragma unroll 1
+                            for (int c = 0; c < 8; c++) {
+                                uint32_t o[16];
+                                ks_ld16(t_o + 16 * c, o);
+                                ks_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+                                ks_st16(t_o + 16 * c, o);
+                            }
+                        }
+                    }
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            const float a = ks_exp2(fmaf(__uint_as_float(v[h][2 * k]), f, -base)), d = ks_exp2(fmaf(__uint_as_float(v[h][2 * k + 1]), f, -base));
+                            s4[k & 3] += a + d;
+                            p[k] = ks_half2(a, d);
+                        }
+                        ks_st16(t_s + 64 * place + 16 * h, p); /* over scores that are in registers */
+                    }
+                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    ks_st_wait();
+                    ks_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.p_full[x][place]);
+                }
+            it += (unsigned)(s.t1 - s.t0);
+            if (ok) {
+                ok = mbar_wait_warp(&bars.unit_done, segments & 1, status);
+                ks_after_sync();
+            }
+            segments++;
+            /* all softmax warps or none go on: what follows has barriers of theirs */
+            if (!ok) atomicCAS(status, PIPE_OK, PIPE_ERR_TMA_WAIT);
+            ks_softmax_sync();
+            if (tid == 0) sh_last = 0;
+            ks_softmax_sync();
+            if (!ok) sh_last = 2;
+            ks_softmax_sync();
+            if (sh_last == 2) { ok = false; break; }
+
+            const bool whole = s.t0 == 0 && s.t1 == s.tiles;
+            auto store = [&](int c, const float (&v)[32], float scale) { /* columns 32 c ..: units 4 c .. 4 c + 3 of values, two groups in turn */
+                __nv_bfloat16* to = out + at + 64 * (c >> 1) + 16 * (c & 1);
+#pragma unroll
+                for (int odd = 0; odd < 2; odd++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int at0 = 16 * h + 4 * k + odd; /* unit 2 h + k / 2, channels 2 (k % 2), + 1 */
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(v[at0] * scale, v[at0 + 2] * scale);
+                            w[k] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
+                        *reinterpret_cast<uint4*>(to + 32 * odd + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+            };
+            const size_t slot = 2 * (size_t)worker + (s.t0 == 0 ? 1 : 0);
+            if (active) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t v[32];
+                    ks_ld32(t_o + 32 * c, v);
+                    ks_ld_wait();
+                    float y[32];
+#pragma unroll
+                    for (int k = 0; k < 32; k++) y[k] = __uint_as_float(v[k]);
+                    if (whole) {
+                        if (live) store(c, y, sum == 0.0f ? 0.0f : 1.0f / sum);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            parts.o[(slot * 32 + 8 * c + k) * KS_SOFTMAX + tid] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                    }
+                }
+                ks_before_sync(); /* the next unit's first product writes where this has been read */
+                if (!whole) {
+                    parts.max[slot * KS_SOFTMAX + tid] = top;
+                    parts.sum[slot * KS_SOFTMAX + tid] = sum;
+                }
+            }
+            if (!whole) {
+                const int w0 = (int)worker_of(s.u0), w1 = (int)worker_of(s.u0 + (unsigned)s.tiles - 1);
+                ks_softmax_sync();
+                if (tid == 0) sh_last = kv4_arrive(parts.arrived + (size_t)s.row0 * cache.kv_heads + s.head, w1 - w0);
+                ks_softmax_sync();
+                if (sh_last && live) {
+                    auto part = [&](int w) { return (size_t)(2 * w + (w == w0)); };
+                    float all = -INFINITY, l = 0.0f;
+#pragma unroll 8
+                    for (int w = w0; w <= w1; w++) all = fmaxf(all, __ldcg(parts.max + part(w) * KS_SOFTMAX + tid));
+                    const float base = all == -INFINITY ? 0.0f : all;
+#pragma unroll 8
+                    for (int w = w0; w <= w1; w++) {
+                        const size_t k = part(w) * KS_SOFTMAX + tid;
+                        l = fmaf(__ldcg(parts.sum + k), ks_exp2(__ldcg(parts.max + k) - base), l);
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        float y[32];
+#pragma unroll
+                        for (int k = 0; k < 32; k++) y[k] = 0.0f;
+#pragma unroll 2
+                        for (int w = w0; w <= w1; w++) {
+                            const float scale = ks_exp2(__ldcg(parts.max + part(w) * KS_SOFTMAX + tid) - base);
+                            float4 v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) v[k] = __ldcg(parts.o + (part(w) * 32 + 8 * c + k) * KS_SOFTMAX + tid);
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                y[4 * k] = fmaf(v[k].x, scale, y[4 * k]);
+                                y[4 * k + 1] = fmaf(v[k].y, scale, y[4 * k + 1]);
+                                y[4 * k + 2] = fmaf(v[k].z, scale, y[4 * k + 2]);
+                                y[4 * k + 3] = fmaf(v[k].w, scale, y[4 * k + 3]);
+                            }
+                        }
+                        store(c, y, l == 0.0f ? 0.0f : 1.0f / l);
+                    }
+                }
+                ks_softmax_sync();
+            }
+            cur += (unsigned)(s.t1 - s.t0);
+        }
+    } else if (warp < 12) {
+        /* ================= pages to operands ================= */
+        const int p = tid - KS_SOFTMAX, g = lane >> 2, t = lane & 3, plane = (p >> 5) & 1;
+        unsigned it = 0;
+        bool ok = true;
+        int chunk = chunk_at;
+        for (unsigned cur = begin; cur < end && ok;) {
+            const Segment s = segment(cur, chunk);
+            const int pages = s.t1 - s.t0;
+            int page_of = -1; /* lane i keeps the (32 n + i)-th */
+            auto page_at = [&](int i) {
+                if ((i & 31) == 0) {
+                    const int pos = (s.t0 + i + lane) * S2P_B200_KV4_PAGE;
+                    page_of = i + lane < pages && pos < s.seen ? kv4_page(cache, s.seq, pos) : -1;
+                }
+                return __shfl_sync(S2P_FULL_MASK, page_of, i & 31);
+            };
+            /* this thread's units are in blocks p >> 6 and 2 + (p >> 6) */
+            uint4 kc[2], kp[2], vc[2], vs[2], vm[2];
+            const uint4 none = make_uint4(0, 0, 0, 0);
+            auto block_of = [&](int page, int j) { return page < 0 ? nullptr : kv4_block(cache, page, s.head, (2 * j + (p >> 6)) * 16); };
+            auto load_keys = [&](int page) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const unsigned char* blk = block_of(page, j);
+                    kc[j] = blk ? *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16) : none;
+                    kp[j] = blk ? *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16) : none;
+                }
+            };
+            auto load_values = [&](int page) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const unsigned char* blk = block_of(page, j);
+                    vc[j] = blk ? *reinterpret_cast<const uint4*>(blk + 1024 + plane * 512 + lane * 16) : none;
+                    vs[j] = blk ? *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16) : none;
+                    vm[j] = blk ? *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16) : none;
+                }
+            };
+            int page = page_at(0);
+            load_keys(page);
+            load_values(page);
+            for (int i = s.t0; i < s.t1; i++, it++) {
+                const unsigned stage = it % KS_STAGES, turn = it / KS_STAGES; /* the turn-th use of the stage */
+                ok = turn == 0 || mbar_wait_warp(&bars.k_free[stage], (turn - 1) & 1, status);
+                if (!ok) break;
+                if (p == 0) sh_absent[it & 7] = page < 0;
+                unsigned char* to = sk + stage * KS_K_BYTES;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + g;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t sw = k < 2 ? kp[j].x : kp[j].y, mw = k < 2 ? kp[j].z : kp[j].w;
+                        const __half2 sc = ks_h2(prmt(sw, sw, (k & 1) ? 0x3232 : 0x1010)), mn = ks_h2(prmt(mw, mw, (k & 1) ? 0x3232 : 0x1010));
+                        *reinterpret_cast<uint4*>(to + (4 * k + t) * KS_K_PITCH + pos * 16) = ks_widen(ks_word(kc[j], k), sc, mn);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.k_full[stage]);
+                const int next = i + 1 < s.t1 ? page_at(i + 1 - s.t0) : -1;
+                load_keys(next);
+                ok = turn == 0 || mbar_wait_warp(&bars.v_free[stage], (turn - 1) & 1, status);
+                if (!ok) break;
+                to = sv + stage * KS_V_BYTES;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + 2 * t;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) { /* positions pos, pos + 1; words of groups 0, 1 and 2, 3 */
+                        const int word = k & 1, second = k >> 1;
+                        const uint32_t sel = second ? 0x7632 : 0x5410;
+                        const __half2 sc = ks_h2(prmt(word ? vs[j].z : vs[j].x, word ? vs[j].w : vs[j].y, sel));
+                        const __half2 mn = ks_h2(prmt(word ? vm[j].z : vm[j].x, word ? vm[j].w : vm[j].y, sel));
+                        uint4 v = ks_widen(ks_word(vc[j], 2 * second + word), sc, mn);
+                        /* nobody has written what lies behind the last position: it must not meet a zero weight as NaN */
+                        if (i * KS_TILE + pos + second >= s.seen) v = none;
+                        *reinterpret_cast<uint4*>(to + (g + 8 * word) * KS_V_PITCH + (pos + second) * 16) = v;
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.v_full[stage]);
+                page = next;
+                load_values(page);
+            }
+            cur += (unsigned)(s.t1 - s.t0);
+        }
+    } else if (begin < end) {
+        /* ================= the products ================= */
+        if (warp_elect()) {
+            /* D f32, A and B f16, M 128, N 64 and 128; B of the second product has its rows (positions) along K: MN-major */
+            const uint32_t idesc = (1u << 4) | (8u << 17) | (8u << 24), idesc_v = (1u << 4) | (16u << 17) | (8u << 24) | (1u << 16);
+            const uint64_t dq = ks_desc(smem_u32(sq), 2048, 128), dk = ks_desc(smem_u32(sk), KS_K_PITCH, 128);
+            const uint64_t dv = ks_desc(smem_u32(sv), 128, KS_V_PITCH);
+            unsigned it = 0, n[2] = {0, 0}, segments = 0; /* n: pages of each row tile whose values have been asked for */
+            bool ok = true;
+            int chunk = chunk_at;
+            auto place_of = [&](int x, unsigned page) { return tmem + 256u + (uint32_t)(x * 128) + 64u * (page & 1); };
+            auto scores = [&](int x, unsigned page, unsigned stage) {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    ks_mma_ss(place_of(x, page), dq + (uint64_t)((x * KS_Q_BYTES + k * 2 * 2048) >> 4), dk + (uint64_t)((stage * KS_K_BYTES + k * 2 * KS_K_PITCH) >> 4),
+                              idesc, k > 0);
+                ks_commit(&bars.s_full[x][page & 1]);
+            };
+            auto values = [&](int x, unsigned page, unsigned stage, bool add) {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    ks_mma_ts(tmem + (uint32_t)(x * 128), place_of(x, page) + 8 * k, dv + (uint64_t)((stage * KS_V_BYTES + k * 256) >> 4), idesc_v, add || k > 0);
+                ks_commit(&bars.o_done[x]);
+            };
+            for (unsigned cur = begin; cur < end && ok; segments++) {
+                const Segment s = segment(cur, chunk);
+                const int tiles = s.t1 - s.t0, two = s.n_rows > tile_rows;
+                ok = mbar_wait_bounded(&bars.q_full, segments & 1, status) && mbar_wait_bounded(&bars.k_full[it % KS_STAGES], (it / KS_STAGES) & 1, status);
+                if (!ok) break;
+                ks_after_sync();
+                for (int x = 0; x <= two; x++) scores(x, n[x], it % KS_STAGES);
+                ks_commit(&bars.k_free[it % KS_STAGES]);
+                for (int i = 0; i < tiles && ok; i++, it++) {
+                    const unsigned stage = it % KS_STAGES, next = (it + 1) % KS_STAGES;
+                    if (i + 1 < tiles) { /* the next scores take the place of the weights before these */
+                        ok = mbar_wait_bounded(&bars.k_full[next], ((it + 1) / KS_STAGES) & 1, status);
+                        for (int x = 0; x <= two && ok; x++) {
+                            if (i > 0) ok = mbar_wait_bounded(&bars.o_done[x], (n[x] - 1) & 1, status);
+                            if (!ok) break;
+                            ks_after_sync();
+                            scores(x, n[x] + 1, next);
+                        }
+                        if (!ok) break;
+                        ks_commit(&bars.k_free[next]);
+                    }
+                    ok = mbar_wait_bounded(&bars.v_full[stage], (it / KS_STAGES) & 1, status);
+                    for (int x = 0; x <= two && ok; x++) {
+                        ok = mbar_wait_bounded(&bars.p_full[x][n[x] & 1], (n[x] >> 1) & 1, status);
+                        if (!ok) break;
+                        ks_after_sync();
+                        values(x, n[x], stage, i > 0);
+                        n[x]++;
+                    }
+                    if (ok) ks_commit(&bars.v_free[stage]);
+                }
+                if (ok) ks_commit(&bars.unit_done);
+                cur += (unsigned)tiles;
+            }
+            /* TMEM must not be freed under products in flight: they complete by themselves, and this waits for them with a limit of its own */
+            ks_commit(&bars.all_done);
+            PipeDeadline dl;
+            for (unsigned i = 0; i < PIPE_MBAR_TRIES && !mbar_try_wait(&bars.all_done, 0); i++)
+                if ((i & 63u) == 63u && dl.expired(2000000000ull)) break;
+        }
+        __syncwarp();
+    }
+    ks_before_sync();
+    __syncthreads();
+    ks_after_sync();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+/* chunks that the batch can have: its rows in units, and a broken one for each entry */
+static int ks_chunks(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b) {
+    const int unit = 2 * (KS_ROWS / (c->q_heads / c->kv_heads));
+    const long long most = (long long)b->rows / unit + (b->n < b->rows ? b->n : b->rows);
+    return most < (1 << 20) ? (int)most : 1 << 20;
+}
+constexpr int KS_MOST_SMEM = 225 * 1024;
+
+extern "C" int kv4_slices_serve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b) {
+    return KS_OPERANDS + ks_line_bytes(ks_chunks(c, b), b->n) <= (size_t)KS_MOST_SMEM;
+}
+
+extern "C" cudaError_t kv4_slices(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, int few, const void* q, void* out, cudaStream_t st) {
+    static bool attr_set[64] = {false};
+    static int sms[64] = {0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!attr_set[dev]) {
+        e = cudaFuncSetAttribute(k_kv4_slices, cudaFuncAttributeMaxDynamicSharedMemorySize, KS_MOST_SMEM);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        attr_set[dev] = true;
+    }
+    KsParts p;
+    unsigned char* area = static_cast<unsigned char*>(c->work) + KV4_STATUS_BYTES;
+    p.status = static_cast<int*>(c->work);
+    p.arrived = reinterpret_cast<unsigned*>(area + kv4_area_bytes(c->n_pages));
+    p.o = reinterpret_cast<float4*>(area);
+    p.max = reinterpret_cast<float*>(area + (size_t)2 * KV4_SLICE_CTAS * KS_SOFTMAX * 128 * sizeof(float));
+    p.sum = p.max + (size_t)2 * KV4_SLICE_CTAS * KS_SOFTMAX;
+    const int grid = sms[dev] < KV4_SLICE_CTAS ? sms[dev] : KV4_SLICE_CTAS;
+    return launch_after(k_kv4_slices, dim3((unsigned)grid), KS_THREADS, KS_OPERANDS + ks_line_bytes(ks_chunks(c, b), b->n), st, kv4_view(*c, layer),
+                        kv4_rows(*b), few, static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), p);
+}
+
+}  // namespace s2p
