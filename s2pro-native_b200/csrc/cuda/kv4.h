@@ -27,7 +27,7 @@ extern "C" {
 
 /* Bytes of the area.  The page operators keep a few words, a pair of pages per move and a new number per page. */
 static inline size_t kv4_area_bytes(int n_pages) {
-    const size_t tokens = (size_t)KV4_PARTS * (128 + 2) * sizeof(float), slices = (size_t)2 * KV4_SLICE_CTAS * 256 * (128 + 2) * sizeof(float);
+    const size_t tokens = (size_t)KV4_PARTS * (128 + 2) * sizeof(float), slices = (size_t)2 * KV4_SLICE_CTAS * (256 * (128 + 2) + 8) * sizeof(float);
     const size_t part = tokens > slices ? tokens : slices;
     const size_t lists = 256 + ((size_t)n_pages / 2 + 1 + S2P_B200_KV4_MAX_LIST) * 8 + (size_t)n_pages * 4;
     return ((part > lists ? part : lists) + 255) / 256 * 256;

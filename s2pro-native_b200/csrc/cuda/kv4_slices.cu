@@ -10,26 +10,28 @@
  * Roles, coupled by mbarriers only:
  *   warps 0..3, 4..7   one thread a query row of the first, second tile: the row as f16 into shared memory (times a power of two, so that its
  *                      largest value is 512..1023: exact), then the softmax with the row's 64 scores in registers, at the end the result
- *   warps 8..11        turn pages into operands: s c + m in f16 (one rounding, 2^-11), keys as [channel / 8][position] units of 8 channels,
- *                      values likewise; codes and parameters of the next page are under way while this one is converted; four stages
+ *   warps 8..11        bring pages into shared memory four ahead (with loads into registers one ahead they waited for half their time) and
+ *                      turn them into operands: s c + m in f16 (one rounding, 2^-11), keys as [channel / 8][position] units of 8
+ *                      channels, values likewise; three stages
  *   warp 12            one thread issues the products.  Each row tile has two places for scores, so the scores of page i + 1 are
  *                      computed while the softmax of page i runs: it never waits for them.
  * Both row tiles use the same converted keys and values, which is what two of them are for.  Every operand is in the unswizzled
  * core-matrix layout (8 rows x 16 bytes); a unit plane has 32 or 16 bytes more than its positions take, so that the converting lanes'
  * stores fall on different banks.
  *
- * Work is cut like that of single tokens: the pages of all units form one line, each CTA takes an equal stretch of it, and
- * the last CTA of a shared unit adds the parts in order. */
+ * Work is cut like that of single tokens: the pages of all units form one line, each CTA takes an equal stretch of it.  The parts of a
+ * shared unit are added, in order, by a second kernel over all SMs: in the last CTA to arrive that took 8 us for two parts of 128 KB and
+ * 20 for five, with the other SMs idle. */
 #include "kv4.cuh"
 #include "pipe.cuh"
 
 namespace s2p {
 
-constexpr int KS_ROWS = 128, KS_TILE = S2P_B200_KV4_PAGE, KS_STAGES = 4, KS_THREADS = 13 * 32, KS_SOFTMAX = 256;
+constexpr int KS_ROWS = 128, KS_TILE = S2P_B200_KV4_PAGE, KS_STAGES = 3, KS_RAW = 5, KS_THREADS = 13 * 32, KS_SOFTMAX = 256;
 constexpr int KS_Q_BYTES = 16 * 128 * 16;                                  /* one row tile: [channel / 8][row] units */
 constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
-constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES);
+constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + KS_RAW * KV4_HEAD_BYTES;
 constexpr int KS_LEAST = 5;                                                /* pages that make a CTA worth its while */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
@@ -43,15 +45,19 @@ struct KsLine { /* in shared memory: the chunks (units of one kv head each) of a
     unsigned* upto;  /* [chunks + 1] position tiles times kv heads before a chunk */
     int* first;      /* [entries + 1] chunks before an entry */
     int* start;      /* [entries + 1] rows before an entry */
+    int *seq, *p0;   /* [entries] its sequence, and its first position or -1 */
 };
-static inline size_t ks_line_bytes(int chunks, int n) { return (size_t)(chunks + 1 + 2 * (n + 1)) * 4; }
+static inline size_t ks_line_bytes(int chunks, int n) { return (size_t)(chunks + 1 + 4 * (n + 1)) * 4; }
 
+/* What a CTA leaves: slot 2 w + 1 where CTA w begins a unit that others end, 2 w where it goes on with one. */
 struct KsParts {
     float *max, *sum; /* [slot][256 rows] */
-    float4* o;        /* [slot][channel / 4][256 rows] */
-    unsigned* arrived;
+    float4* o;        /* [slot][column / 4][256 rows] */
+    int4* unit;       /* [w] the unit that w begins and others end: first row, rows (0: none), kv head, last CTA */
     int* status;
 };
+/* Columns of O are the values' channels in the order of their units: unit u holds channels 64 (u / 8) + 4 (u % 8) + 0 .. 3 in its even places and
+ * the same + 32 in its odd ones. */
 
 __device__ __forceinline__ uint64_t ks_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
@@ -94,7 +100,13 @@ __device__ __forceinline__ void ks_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-__device__ __forceinline__ void ks_softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+/* Waits of this kernel: what polls is four instructions, and what happens otherwise is out of line.  (mbar_wait_bounded written out at
+ * every place cost the issuing thread 0.2 us a wait that was over already: its instructions had to be fetched each time.) */
+__device__ __noinline__ bool ks_wait_on(uint64_t* bar, unsigned parity, int* status) { return mbar_wait_bounded(bar, parity, status); }
+__device__ __forceinline__ bool ks_wait(uint64_t* bar, unsigned parity, int* status) { return mbar_try_wait(bar, parity) || ks_wait_on(bar, parity, status); }
+__device__ __forceinline__ bool ks_wait_warp(uint64_t* bar, unsigned parity, int* status) { return __all_sync(S2P_FULL_MASK, ks_wait(bar, parity, status)); }
+template <int X> struct KsTile { static constexpr int value = X; };
+__device__ __forceinline__ void ks_pages_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ float ks_exp2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -125,16 +137,18 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ KsBars bars;
     __shared__ uint32_t sh_tmem;
-    __shared__ unsigned sh_scan[13], sh_last;
-    __shared__ int sh_absent[8];
+    __shared__ unsigned sh_scan[13];
+    __shared__ int sh_absent[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = cache.q_heads / cache.kv_heads, tile_rows = KS_ROWS / group, unit_rows = 2 * tile_rows;
     const int capacity = cache.stride * S2P_B200_KV4_PAGE;
-    unsigned char *sq = smem, *sk = sq + 2 * KS_Q_BYTES, *sv = sk + KS_STAGES * KS_K_BYTES;
+    unsigned char *sq = smem, *sk = sq + 2 * KS_Q_BYTES, *sv = sk + KS_STAGES * KS_K_BYTES, *raw = sv + KS_STAGES * KS_V_BYTES;
     KsLine line;
     line.first = reinterpret_cast<int*>(smem + KS_OPERANDS);
     line.start = line.first + b.n + 1;
-    line.upto = reinterpret_cast<unsigned*>(line.start + b.n + 1);
+    line.seq = line.start + b.n + 1;
+    line.p0 = line.seq + b.n + 1;
+    line.upto = reinterpret_cast<unsigned*>(line.p0 + b.n + 1);
     int* status = parts.status;
 
     if (warp == 12) {
@@ -187,7 +201,15 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     const int per = b.n / KS_THREADS + 1;
     {
         int top = 0; /* starts made ascending and kept inside the activations, whatever row0 holds */
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) top = max(top, line.start[e] = min(b.row0[e], b.rows));
+        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
+            const int r = b.row0[e];
+            if (e < b.n) {
+                const int seq = b.seqs[e], p0 = b.pos0[e];
+                line.seq[e] = seq;
+                line.p0[e] = (unsigned)seq < (unsigned)cache.max_seqs && p0 <= (1 << 30) ? p0 : -1;
+            }
+            top = max(top, line.start[e] = min(r, b.rows));
+        }
         int before = top;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -207,7 +229,6 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh_tmem);
     auto rows_of = [&](int e) { return line.start[e + 1] - line.start[e]; };
     auto chunks_of = [&](int e) { return rows_of(e) > few ? (rows_of(e) + unit_rows - 1) / unit_rows : 0; };
-    auto first_of = [&](int e) { return (unsigned)b.seqs[e] < (unsigned)cache.max_seqs && b.pos0[e] <= (1 << 30) ? b.pos0[e] : -1; };
     auto seen_by = [&](int p0, int row) { return p0 < 0 ? 0 : (int)min((long long)p0 + row + 1, (long long)capacity); };
     unsigned chunks, total;
     {
@@ -230,7 +251,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     };
     auto tiles_of = [&](int e, int chunk) { /* position tiles of a chunk's unit */
         const int last = min(rows_of(e), (chunk - line.first[e] + 1) * unit_rows) - 1;
-        return max(1, (seen_by(first_of(e), last) + KS_TILE - 1) / KS_TILE);
+        return max(1, (seen_by(line.p0[e], last) + KS_TILE - 1) / KS_TILE);
     };
     {
         const int each = (int)chunks / KS_THREADS + 1;
@@ -279,21 +300,22 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         s.r0 = (chunk - line.first[s.e]) * unit_rows;
         s.n_rows = min(unit_rows, rows_of(s.e) - s.r0);
         s.row0 = line.start[s.e] + s.r0;
-        s.seq = b.seqs[s.e];
-        s.p0 = first_of(s.e);
+        s.seq = line.seq[s.e];
+        s.p0 = line.p0[s.e];
         s.seen = seen_by(s.p0, s.r0 + s.n_rows - 1);
         return s;
     };
 
-    if (warp < 8) {
+    if (begin >= end && tid == 0) parts.unit[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (warp < 8 && begin < end) {
         /* ================= softmax ================= */
         const int x = warp >> 2, r = tid & 127; /* row tile, row */
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_o = tmem + (uint32_t)(x * 128) + lanes, t_s = tmem + 256u + (uint32_t)(x * 128) + lanes;
         unsigned n_s = 0, segments = 0; /* pages of this row tile so far */
-        bool ok = true;
+        bool ok = true, begun = false;
         int chunk = chunk_at;
-        unsigned it = 0; /* position tiles of the CTA so far */
+        unsigned it = 0; /* pages of the CTA so far */
         for (unsigned cur = begin; cur < end && ok;) {
             const Segment s = segment(cur, chunk);
             const int my_row = x * tile_rows + r / group, my_head = s.head * group + r % group;
@@ -332,13 +354,13 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             if (active)
                 for (int i = s.t0; i < s.t1; i++, n_s++) {
                     const unsigned place = n_s & 1;
-                    ok = mbar_wait_warp(&bars.s_full[x][place], (n_s >> 1) & 1, status);
+                    ok = ks_wait_warp(&bars.s_full[x][place], (n_s >> 1) & 1, status);
                     if (!ok) break;
                     ks_after_sync();
                     uint32_t v[2][32];
                     ks_ld32(t_s + 64 * place, v[0]);
                     ks_ld32(t_s + 64 * place + 32, v[1]);
-                    const int left = *reinterpret_cast<volatile int*>(&sh_absent[(it + (unsigned)(i - s.t0)) & 7]) ? 0 : limit - i * KS_TILE;
+                    const int left = *reinterpret_cast<volatile int*>(&sh_absent[(it + (unsigned)(i - s.t0)) & 15]) ? 0 : limit - i * KS_TILE;
                     ks_ld_wait();
                     if (__any_sync(S2P_FULL_MASK, left < KS_TILE)) {
 #pragma unroll
@@ -354,7 +376,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                         top = now;
                         sum *= shrink;
                         if (i > s.t0) { /* behind the product of the page before; the one before that was waited for in front of these scores */
-                            ok = mbar_wait_warp(&bars.o_done[x], (n_s - 1) & 1, status);
+                            ok = ks_wait_warp(&bars.o_done[x], (n_s - 1) & 1, status);
                             if (!ok) break;
                             ks_after_sync();
 #pragma unroll 1
@@ -389,18 +411,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 }
             it += (unsigned)(s.t1 - s.t0);
             if (ok) {
-                ok = mbar_wait_warp(&bars.unit_done, segments & 1, status);
+                ok = ks_wait_warp(&bars.unit_done, segments & 1, status);
                 ks_after_sync();
             }
             segments++;
-            /* all softmax warps or none go on: what follows has barriers of theirs */
-            if (!ok) atomicCAS(status, PIPE_OK, PIPE_ERR_TMA_WAIT);
-            ks_softmax_sync();
-            if (tid == 0) sh_last = 0;
-            ks_softmax_sync();
-            if (!ok) sh_last = 2;
-            ks_softmax_sync();
-            if (sh_last == 2) { ok = false; break; }
+            if (!ok) break; /* the other warps' waits give up by themselves: the status word is set */
 
             const bool whole = s.t0 == 0 && s.t1 == s.tiles;
             auto store = [&](int c, const float (&v)[32], float scale) { /* columns 32 c ..: units 4 c .. 4 c + 3 of values, two groups in turn */
@@ -443,136 +458,106 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     parts.sum[slot * KS_SOFTMAX + tid] = sum;
                 }
             }
-            if (!whole) {
-                const int w0 = (int)worker_of(s.u0), w1 = (int)worker_of(s.u0 + (unsigned)s.tiles - 1);
-                ks_softmax_sync();
-                if (tid == 0) sh_last = kv4_arrive(parts.arrived + (size_t)s.row0 * cache.kv_heads + s.head, w1 - w0);
-                ks_softmax_sync();
-                if (sh_last && live) {
-                    auto part = [&](int w) { return (size_t)(2 * w + (w == w0)); };
-                    float all = -INFINITY, l = 0.0f;
-#pragma unroll 8
-                    for (int w = w0; w <= w1; w++) all = fmaxf(all, __ldcg(parts.max + part(w) * KS_SOFTMAX + tid));
-                    const float base = all == -INFINITY ? 0.0f : all;
-#pragma unroll 8
-                    for (int w = w0; w <= w1; w++) {
-                        const size_t k = part(w) * KS_SOFTMAX + tid;
-                        l = fmaf(__ldcg(parts.sum + k), ks_exp2(__ldcg(parts.max + k) - base), l);
-                    }
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        float y[32];
-#pragma unroll
-                        for (int k = 0; k < 32; k++) y[k] = 0.0f;
-#pragma unroll 2
-                        for (int w = w0; w <= w1; w++) {
-                            const float scale = ks_exp2(__ldcg(parts.max + part(w) * KS_SOFTMAX + tid) - base);
-                            float4 v[8];
-#pragma unroll
-                            for (int k = 0; k < 8; k++) v[k] = __ldcg(parts.o + (part(w) * 32 + 8 * c + k) * KS_SOFTMAX + tid);
-#pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                y[4 * k] = fmaf(v[k].x, scale, y[4 * k]);
-                                y[4 * k + 1] = fmaf(v[k].y, scale, y[4 * k + 1]);
-                                y[4 * k + 2] = fmaf(v[k].z, scale, y[4 * k + 2]);
-                                y[4 * k + 3] = fmaf(v[k].w, scale, y[4 * k + 3]);
-                            }
-                        }
-                        store(c, y, l == 0.0f ? 0.0f : 1.0f / l);
-                    }
-                }
-                ks_softmax_sync();
-            }
+            if (tid == 0 && s.t0 == 0 && !whole) parts.unit[worker] = make_int4(s.row0, s.n_rows, s.head, (int)worker_of(s.u0 + (unsigned)s.tiles - 1));
+            begun |= s.t0 == 0 && !whole;
             cur += (unsigned)(s.t1 - s.t0);
         }
-    } else if (warp < 12) {
+        if (tid == 0 && !begun) parts.unit[worker] = make_int4(0, 0, 0, 0);
+    } else if (warp >= 8 && warp < 12) {
         /* ================= pages to operands ================= */
         const int p = tid - KS_SOFTMAX, g = lane >> 2, t = lane & 3, plane = (p >> 5) & 1;
-        unsigned it = 0;
         bool ok = true;
+        /* what to bring: its own walk along the stretch, KS_RAW - 1 pages ahead of the conversion */
+        unsigned f_cur = begin, f_it = 0;
+        int f_chunk = chunk_at, f_i = 0, page_of = -1; /* lane i keeps the (32 n + i)-th page of the segment */
+        Segment f;
+        f.t0 = f.t1 = 0;
+        auto bring = [&]() {
+            if (f_i == f.t1 - f.t0 && f_cur < end) {
+                f = segment(f_cur, f_chunk);
+                f_cur += (unsigned)(f.t1 - f.t0);
+                f_i = 0;
+            }
+            if (f_i < f.t1 - f.t0) {
+                if ((f_i & 31) == 0) {
+                    const int pos = (f.t0 + f_i + lane) * S2P_B200_KV4_PAGE;
+                    page_of = f_i + lane < f.t1 - f.t0 && pos < f.seen ? kv4_page(cache, f.seq, pos) : -1;
+                }
+                const int page = __shfl_sync(S2P_FULL_MASK, page_of, f_i & 31);
+                if (page >= 0) {
+                    const unsigned char* src = kv4_block(cache, page, f.head, 0) + p * 16;
+                    const uint32_t dst = smem_u32(raw) + f_it % KS_RAW * KV4_HEAD_BYTES + p * 16;
+#pragma unroll
+                    for (int k = 0; k < KV4_HEAD_BYTES / 2048; k++)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 2048), "l"(src + k * 2048) : "memory");
+                }
+                if (p == 0) sh_absent[f_it & 15] = page < 0;
+                f_i++;
+                f_it++;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int i = 0; i < KS_RAW - 1; i++) bring();
+        unsigned it = 0;
         int chunk = chunk_at;
         for (unsigned cur = begin; cur < end && ok;) {
             const Segment s = segment(cur, chunk);
-            const int pages = s.t1 - s.t0;
-            int page_of = -1; /* lane i keeps the (32 n + i)-th */
-            auto page_at = [&](int i) {
-                if ((i & 31) == 0) {
-                    const int pos = (s.t0 + i + lane) * S2P_B200_KV4_PAGE;
-                    page_of = i + lane < pages && pos < s.seen ? kv4_page(cache, s.seq, pos) : -1;
-                }
-                return __shfl_sync(S2P_FULL_MASK, page_of, i & 31);
-            };
-            /* this thread's units are in blocks p >> 6 and 2 + (p >> 6) */
-            uint4 kc[2], kp[2], vc[2], vs[2], vm[2];
-            const uint4 none = make_uint4(0, 0, 0, 0);
-            auto block_of = [&](int page, int j) { return page < 0 ? nullptr : kv4_block(cache, page, s.head, (2 * j + (p >> 6)) * 16); };
-            auto load_keys = [&](int page) {
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const unsigned char* blk = block_of(page, j);
-                    kc[j] = blk ? *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16) : none;
-                    kp[j] = blk ? *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16) : none;
-                }
-            };
-            auto load_values = [&](int page) {
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const unsigned char* blk = block_of(page, j);
-                    vc[j] = blk ? *reinterpret_cast<const uint4*>(blk + 1024 + plane * 512 + lane * 16) : none;
-                    vs[j] = blk ? *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16) : none;
-                    vm[j] = blk ? *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16) : none;
-                }
-            };
-            int page = page_at(0);
-            load_keys(page);
-            load_values(page);
             for (int i = s.t0; i < s.t1; i++, it++) {
                 const unsigned stage = it % KS_STAGES, turn = it / KS_STAGES; /* the turn-th use of the stage */
-                ok = turn == 0 || mbar_wait_warp(&bars.k_free[stage], (turn - 1) & 1, status);
-                if (!ok) break;
-                if (p == 0) sh_absent[it & 7] = page < 0;
+                asm volatile("cp.async.wait_group %0;" ::"n"(KS_RAW - 2) : "memory");
+                ks_pages_sync(); /* everybody's share of this page has come, and everybody is done with the one before it: */
+                bring();         /* ... its place is free */
+                const bool absent = *reinterpret_cast<volatile int*>(&sh_absent[it & 15]) != 0;
+                const unsigned char* page = raw + it % KS_RAW * KV4_HEAD_BYTES;
+                /* a wait that has given up once is not waited for again, but the barriers above need every warp */
+                ok = ok && (turn == 0 || ks_wait_warp(&bars.k_free[stage], (turn - 1) & 1, status));
                 unsigned char* to = sk + stage * KS_K_BYTES;
+                if (ok) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + g;
+                    for (int j = 0; j < 2; j++) { /* this thread's units are in blocks p >> 6 and 2 + (p >> 6) */
+                        const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
+                        const uint4 kc = *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16), kp = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16);
+                        const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + g;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t sw = k < 2 ? kp[j].x : kp[j].y, mw = k < 2 ? kp[j].z : kp[j].w;
-                        const __half2 sc = ks_h2(prmt(sw, sw, (k & 1) ? 0x3232 : 0x1010)), mn = ks_h2(prmt(mw, mw, (k & 1) ? 0x3232 : 0x1010));
-                        *reinterpret_cast<uint4*>(to + (4 * k + t) * KS_K_PITCH + pos * 16) = ks_widen(ks_word(kc[j], k), sc, mn);
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t sw = k < 2 ? kp.x : kp.y, mw = k < 2 ? kp.z : kp.w;
+                            const __half2 sc = ks_h2(prmt(sw, sw, (k & 1) ? 0x3232 : 0x1010)), mn = ks_h2(prmt(mw, mw, (k & 1) ? 0x3232 : 0x1010));
+                            *reinterpret_cast<uint4*>(to + (4 * k + t) * KS_K_PITCH + pos * 16) = ks_widen(ks_word(kc, k), sc, mn);
+                        }
                     }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.k_full[stage]);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.k_full[stage]);
-                const int next = i + 1 < s.t1 ? page_at(i + 1 - s.t0) : -1;
-                load_keys(next);
-                ok = turn == 0 || mbar_wait_warp(&bars.v_free[stage], (turn - 1) & 1, status);
-                if (!ok) break;
+                ok = ok && (turn == 0 || ks_wait_warp(&bars.v_free[stage], (turn - 1) & 1, status));
                 to = sv + stage * KS_V_BYTES;
+                if (ok) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + 2 * t;
+                    for (int j = 0; j < 2; j++) {
+                        const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
+                        const uint4 vc = *reinterpret_cast<const uint4*>(blk + 1024 + plane * 512 + lane * 16);
+                        const uint4 vs = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16), vm = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16);
+                        const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + 2 * t;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) { /* positions pos, pos + 1; words of groups 0, 1 and 2, 3 */
-                        const int word = k & 1, second = k >> 1;
-                        const uint32_t sel = second ? 0x7632 : 0x5410;
-                        const __half2 sc = ks_h2(prmt(word ? vs[j].z : vs[j].x, word ? vs[j].w : vs[j].y, sel));
-                        const __half2 mn = ks_h2(prmt(word ? vm[j].z : vm[j].x, word ? vm[j].w : vm[j].y, sel));
-                        uint4 v = ks_widen(ks_word(vc[j], 2 * second + word), sc, mn);
-                        /* nobody has written what lies behind the last position: it must not meet a zero weight as NaN */
-                        if (i * KS_TILE + pos + second >= s.seen) v = none;
-                        *reinterpret_cast<uint4*>(to + (g + 8 * word) * KS_V_PITCH + (pos + second) * 16) = v;
+                        for (int k = 0; k < 4; k++) { /* positions pos, pos + 1; words of groups 0, 1 and 2, 3 */
+                            const int word = k & 1, second = k >> 1;
+                            const uint32_t sel = second ? 0x7632 : 0x5410;
+                            const __half2 sc = ks_h2(prmt(word ? vs.z : vs.x, word ? vs.w : vs.y, sel));
+                            const __half2 mn = ks_h2(prmt(word ? vm.z : vm.x, word ? vm.w : vm.y, sel));
+                            uint4 v = ks_widen(ks_word(vc, 2 * second + word), sc, mn);
+                            /* nobody has written what lies behind the last position: it must not meet a zero weight as NaN */
+                            if (absent || i * KS_TILE + pos + second >= s.seen) v = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(to + (g + 8 * word) * KS_V_PITCH + (pos + second) * 16) = v;
+                        }
                     }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.v_full[stage]);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.v_full[stage]);
-                page = next;
-                load_values(page);
             }
             cur += (unsigned)(s.t1 - s.t0);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (begin < end) {
         /* ================= the products ================= */
         if (warp_elect()) {
@@ -580,53 +565,70 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             const uint32_t idesc = (1u << 4) | (8u << 17) | (8u << 24), idesc_v = (1u << 4) | (16u << 17) | (8u << 24) | (1u << 16);
             const uint64_t dq = ks_desc(smem_u32(sq), 2048, 128), dk = ks_desc(smem_u32(sk), KS_K_PITCH, 128);
             const uint64_t dv = ks_desc(smem_u32(sv), 128, KS_V_PITCH);
-            unsigned it = 0, n[2] = {0, 0}, segments = 0; /* n: pages of each row tile whose values have been asked for */
+            unsigned stage = 0, turn = 0, n0 = 0, n1 = 0, segments = 0; /* n0, n1: pages of each row tile whose values have been asked for */
             bool ok = true;
             int chunk = chunk_at;
-            auto place_of = [&](int x, unsigned page) { return tmem + 256u + (uint32_t)(x * 128) + 64u * (page & 1); };
-            auto scores = [&](int x, unsigned page, unsigned stage) {
+            /* Both row tiles are written out: with the tile as a loop's variable the compiler kept what the products take in ordinary registers, and a
+             * page's 24 products took 1.6 us to issue (their rate is 0.7). */
+            auto scores = [&](auto tile, unsigned page, unsigned from) {
+                constexpr int x = decltype(tile)::value;
+                const uint32_t d = tmem + 256u + x * 128 + 64u * (page & 1);
+                const uint64_t keys = dk + (uint64_t)(from * (KS_K_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    ks_mma_ss(place_of(x, page), dq + (uint64_t)((x * KS_Q_BYTES + k * 2 * 2048) >> 4), dk + (uint64_t)((stage * KS_K_BYTES + k * 2 * KS_K_PITCH) >> 4),
-                              idesc, k > 0);
+                for (int k = 0; k < 8; k++) ks_mma_ss(d, dq + (uint64_t)((x * KS_Q_BYTES + k * 2 * 2048) >> 4), keys + (uint64_t)((k * 2 * KS_K_PITCH) >> 4), idesc, k > 0);
                 ks_commit(&bars.s_full[x][page & 1]);
             };
-            auto values = [&](int x, unsigned page, unsigned stage, bool add) {
+            auto values = [&](auto tile, unsigned page, bool add) {
+                constexpr int x = decltype(tile)::value;
+                const uint32_t d = tmem + 256u + x * 128 + 64u * (page & 1);
+                const uint64_t from = dv + (uint64_t)(stage * (KS_V_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    ks_mma_ts(tmem + (uint32_t)(x * 128), place_of(x, page) + 8 * k, dv + (uint64_t)((stage * KS_V_BYTES + k * 256) >> 4), idesc_v, add || k > 0);
+                for (int k = 0; k < 4; k++) ks_mma_ts(tmem + x * 128, d + 8 * k, from + (uint64_t)((k * 256) >> 4), idesc_v, add || k > 0);
                 ks_commit(&bars.o_done[x]);
             };
+            const KsTile<0> first_tile;
+            const KsTile<1> second_tile;
             for (unsigned cur = begin; cur < end && ok; segments++) {
                 const Segment s = segment(cur, chunk);
-                const int tiles = s.t1 - s.t0, two = s.n_rows > tile_rows;
-                ok = mbar_wait_bounded(&bars.q_full, segments & 1, status) && mbar_wait_bounded(&bars.k_full[it % KS_STAGES], (it / KS_STAGES) & 1, status);
+                const int tiles = s.t1 - s.t0;
+                const bool two = s.n_rows > tile_rows;
+                ok = ks_wait(&bars.q_full, segments & 1, status) && ks_wait(&bars.k_full[stage], turn & 1, status);
                 if (!ok) break;
                 ks_after_sync();
-                for (int x = 0; x <= two; x++) scores(x, n[x], it % KS_STAGES);
-                ks_commit(&bars.k_free[it % KS_STAGES]);
-                for (int i = 0; i < tiles && ok; i++, it++) {
-                    const unsigned stage = it % KS_STAGES, next = (it + 1) % KS_STAGES;
+                scores(first_tile, n0, stage);
+                if (two) scores(second_tile, n1, stage);
+                ks_commit(&bars.k_free[stage]);
+                for (int i = 0; i < tiles; i++) {
+                    const unsigned next = stage + 1 == KS_STAGES ? 0 : stage + 1, next_turn = turn + (stage + 1 == KS_STAGES);
                     if (i + 1 < tiles) { /* the next scores take the place of the weights before these */
-                        ok = mbar_wait_bounded(&bars.k_full[next], ((it + 1) / KS_STAGES) & 1, status);
-                        for (int x = 0; x <= two && ok; x++) {
-                            if (i > 0) ok = mbar_wait_bounded(&bars.o_done[x], (n[x] - 1) & 1, status);
-                            if (!ok) break;
-                            ks_after_sync();
-                            scores(x, n[x] + 1, next);
-                        }
-                        if (!ok) break;
-                        ks_commit(&bars.k_free[next]);
-                    }
-                    ok = mbar_wait_bounded(&bars.v_full[stage], (it / KS_STAGES) & 1, status);
-                    for (int x = 0; x <= two && ok; x++) {
-                        ok = mbar_wait_bounded(&bars.p_full[x][n[x] & 1], (n[x] >> 1) & 1, status);
+                        ok = ks_wait(&bars.k_full[next], next_turn & 1, status);
+                        if (ok && i > 0) ok = ks_wait(&bars.o_done[0], (n0 - 1) & 1, status);
                         if (!ok) break;
                         ks_after_sync();
-                        values(x, n[x], stage, i > 0);
-                        n[x]++;
+                        scores(first_tile, n0 + 1, next);
+                        if (two) {
+                            if (i > 0) ok = ks_wait(&bars.o_done[1], (n1 - 1) & 1, status);
+                            if (!ok) break;
+                            ks_after_sync();
+                            scores(second_tile, n1 + 1, next);
+                        }
+                        ks_commit(&bars.k_free[next]);
                     }
-                    if (ok) ks_commit(&bars.v_free[stage]);
+                    ok = ks_wait(&bars.v_full[stage], turn & 1, status) && ks_wait(&bars.p_full[0][n0 & 1], (n0 >> 1) & 1, status);
+                    if (!ok) break;
+                    ks_after_sync();
+                    values(first_tile, n0, i > 0);
+                    n0++;
+                    if (two) {
+                        ok = ks_wait(&bars.p_full[1][n1 & 1], (n1 >> 1) & 1, status);
+                        if (!ok) break;
+                        ks_after_sync();
+                        values(second_tile, n1, i > 0);
+                        n1++;
+                    }
+                    ks_commit(&bars.v_free[stage]);
+                    stage = next;
+                    turn = next_turn;
                 }
                 if (ok) ks_commit(&bars.unit_done);
                 cur += (unsigned)tiles;
@@ -643,6 +645,63 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     __syncthreads();
     ks_after_sync();
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+/* The parts of shared units, in order of the CTAs that left them.  Block (w, y): 16 rows of the unit that CTA w began; a thread has two units of
+ * channels of a row, and four parts' loads are under way at a time. */
+constexpr int KS_JOIN_ROWS = 16, KS_JOIN_THREADS = 128;
+__global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int q_heads, int group, __nv_bfloat16* out) {
+    grid_wait();
+    grid_release();
+    const int w0 = blockIdx.x, r = blockIdx.y * KS_JOIN_ROWS + (threadIdx.x & 15), u = threadIdx.x >> 4;
+    const int4 unit = parts.unit[w0];
+    const int tile_rows = KS_ROWS / group, x = r / KS_ROWS, in = r % KS_ROWS, row = x * tile_rows + in / group;
+    if (in >= tile_rows * group || row >= unit.y) return;
+    const int w1 = unit.w;
+    float top = -INFINITY, sum = 0.0f, y[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) y[k] = 0.0f;
+    for (int w = w0; w <= w1; w += 4) {
+        float m[4], l[4];
+        float4 v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool there = w + i <= w1;
+            const size_t slot = (size_t)(2 * (w + i) + (w + i == w0));
+            m[i] = there ? __ldcg(parts.max + slot * KS_SOFTMAX + r) : -INFINITY;
+            l[i] = there ? __ldcg(parts.sum + slot * KS_SOFTMAX + r) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) /* units u and u + 8 */
+                v[i][k] = there ? __ldcg(parts.o + (slot * 32 + 2 * u + (k & 1) + 16 * (k >> 1)) * KS_SOFTMAX + r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), base = now == -INFINITY ? 0.0f : now, keep = ks_exp2(top - base);
+        sum *= keep;
+#pragma unroll
+        for (int k = 0; k < 16; k++) y[k] *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float scale = ks_exp2(m[i] - base);
+            sum = fmaf(l[i], scale, sum);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                y[4 * k] = fmaf(v[i][k].x, scale, y[4 * k]);
+                y[4 * k + 1] = fmaf(v[i][k].y, scale, y[4 * k + 1]);
+                y[4 * k + 2] = fmaf(v[i][k].z, scale, y[4 * k + 2]);
+                y[4 * k + 3] = fmaf(v[i][k].w, scale, y[4 * k + 3]);
+            }
+        }
+        top = now;
+    }
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+    __nv_bfloat16* to = out + ((size_t)(unit.x + row) * q_heads + unit.z * group + in % group) * 128 + 4 * u;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int odd = 0; odd < 2; odd++) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(y[8 * h + odd] * scale, y[8 * h + 2 + odd] * scale),
+                                 d = __floats2bfloat162_rn(y[8 * h + 4 + odd] * scale, y[8 * h + 6 + odd] * scale);
+            *reinterpret_cast<uint2*>(to + 64 * h + 32 * odd) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&d));
+        }
 }
 
 /* chunks that the batch can have: its rows in units, and a broken one for each entry */
@@ -673,13 +732,17 @@ extern "C" cudaError_t kv4_slices(const s2p_b200_kv4* c, const s2p_b200_kv4_batc
     KsParts p;
     unsigned char* area = static_cast<unsigned char*>(c->work) + KV4_STATUS_BYTES;
     p.status = static_cast<int*>(c->work);
-    p.arrived = reinterpret_cast<unsigned*>(area + kv4_area_bytes(c->n_pages));
     p.o = reinterpret_cast<float4*>(area);
     p.max = reinterpret_cast<float*>(area + (size_t)2 * KV4_SLICE_CTAS * KS_SOFTMAX * 128 * sizeof(float));
     p.sum = p.max + (size_t)2 * KV4_SLICE_CTAS * KS_SOFTMAX;
+    p.unit = reinterpret_cast<int4*>(p.sum + (size_t)2 * KV4_SLICE_CTAS * KS_SOFTMAX);
     const int grid = sms[dev] < KV4_SLICE_CTAS ? sms[dev] : KV4_SLICE_CTAS;
-    return launch_after(k_kv4_slices, dim3((unsigned)grid), KS_THREADS, KS_OPERANDS + ks_line_bytes(ks_chunks(c, b), b->n), st, kv4_view(*c, layer),
-                        kv4_rows(*b), few, static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), p);
+    const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
+    __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out);
+    e = launch_after(k_kv4_slices, dim3((unsigned)grid), KS_THREADS, KS_OPERANDS + ks_line_bytes(ks_chunks(c, b), b->n), st, kv4_view(*c, layer),
+                     kv4_rows(*b), few, qb, ob, p);
+    if (e != cudaSuccess) return e;
+    return launch_after(k_kv4_join, dim3((unsigned)grid, KS_SOFTMAX / KS_JOIN_ROWS), KS_JOIN_THREADS, 0, st, p, c->q_heads, c->q_heads / c->kv_heads, ob);
 }
 
 }  // namespace s2p
