@@ -10,10 +10,10 @@
  * Roles, coupled by mbarriers only:
  *   warps 0..3, 4..7   one thread a query row of the first, second tile: the row as f16 into shared memory (times a power of two, so that its
  *                      largest value is 512..1023: exact), then the softmax with the row's 64 scores in registers, at the end the result
- *   warps 8..11        bring pages into shared memory four ahead (with loads into registers one ahead they waited for half their time) and
- *                      turn them into operands: s c + m in f16 (one rounding, 2^-11), keys as [channel / 8][position] units of 8
+ *   warps 8..11, 12..15  every other page each: bring it into shared memory (with loads into registers, one page ahead, they waited for half their
+ *                      time; one team of four warps alone took 1.4 us a page, twice what the products need) and turn it into operands: s c + m in f16 (one rounding, 2^-11), keys as [channel / 8][position] units of 8
  *                      channels, values likewise; three stages
- *   warp 12            one thread issues the products.  Each row tile has two places for scores, so the scores of page i + 1 are
+ *   warps 16, 17       one thread each issues a row tile's products.  Each row tile has two places for scores, so the scores of page i + 1 are
  *                      computed while the softmax of page i runs: it never waits for them.
  * Both row tiles use the same converted keys and values, which is what two of them are for.  Every operand is in the unswizzled
  * core-matrix layout (8 rows x 16 bytes); a unit plane has 32 or 16 bytes more than its positions take, so that the converting lanes'
@@ -27,18 +27,18 @@
 
 namespace s2p {
 
-constexpr int KS_ROWS = 128, KS_TILE = S2P_B200_KV4_PAGE, KS_STAGES = 3, KS_RAW = 5, KS_THREADS = 13 * 32, KS_SOFTMAX = 256;
+constexpr int KS_ROWS = 128, KS_TILE = S2P_B200_KV4_PAGE, KS_STAGES = 3, KS_RAW = 2, KS_WARPS = 20, KS_THREADS = KS_WARPS * 32, KS_SOFTMAX = 256;
 constexpr int KS_Q_BYTES = 16 * 128 * 16;                                  /* one row tile: [channel / 8][row] units */
 constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
-constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + KS_RAW * KV4_HEAD_BYTES;
+constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + 2 * KS_RAW * KV4_HEAD_BYTES;
 constexpr int KS_LEAST = 5;                                                /* pages that make a CTA worth its while */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
 struct KsBars {
     uint64_t k_full[KS_STAGES], k_free[KS_STAGES], v_full[KS_STAGES], v_free[KS_STAGES];
     uint64_t s_full[2][2], p_full[2][2]; /* [row tile][place] */
-    uint64_t o_done[2], q_full, unit_done, all_done;
+    uint64_t o_done[2], q_full, unit_done, all_done[2];
 };
 
 struct KsLine { /* in shared memory: the chunks (units of one kv head each) of all entries */
@@ -100,13 +100,22 @@ __device__ __forceinline__ void ks_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-/* Waits of this kernel: what polls is four instructions, and what happens otherwise is out of line.  (mbar_wait_bounded written out at
- * every place cost the issuing thread 0.2 us a wait that was over already: its instructions had to be fetched each time.) */
-__device__ __noinline__ bool ks_wait_on(uint64_t* bar, unsigned parity, int* status) { return mbar_wait_bounded(bar, parity, status); }
-__device__ __forceinline__ bool ks_wait(uint64_t* bar, unsigned parity, int* status) { return mbar_try_wait(bar, parity) || ks_wait_on(bar, parity, status); }
+/* Waits of this kernel: mbar_wait_bounded (pipe.cuh) with the case that nothing has to be waited for in front and the rest out of its way.  (As it
+ * stands there, written out at every place, it cost the issuing thread 0.2 us a wait that was over already: its instructions had to be fetched
+ * each time.) */
+__device__ __forceinline__ bool ks_wait(uint64_t* bar, unsigned parity, int* status) {
+    if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+    const unsigned long long t0 = pipe_now();
+    for (unsigned i = 1; !mbar_try_wait(bar, parity); i++)
+        if ((i & 63u) == 0 && (status_peek(status) != PIPE_OK || pipe_now() - t0 > c_pipe_wait_ns || i >= PIPE_MBAR_TRIES)) {
+            atomicCAS(status, PIPE_OK, PIPE_ERR_TMA_WAIT);
+            return false;
+        }
+    return true;
+}
 __device__ __forceinline__ bool ks_wait_warp(uint64_t* bar, unsigned parity, int* status) { return __all_sync(S2P_FULL_MASK, ks_wait(bar, parity, status)); }
 template <int X> struct KsTile { static constexpr int value = X; };
-__device__ __forceinline__ void ks_pages_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void ks_pages_sync(int team) { asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory"); }
 __device__ __forceinline__ float ks_exp2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -137,7 +146,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ KsBars bars;
     __shared__ uint32_t sh_tmem;
-    __shared__ unsigned sh_scan[13];
+    __shared__ unsigned sh_scan[KS_WARPS];
     __shared__ int sh_absent[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = cache.q_heads / cache.kv_heads, tile_rows = KS_ROWS / group, unit_rows = 2 * tile_rows;
@@ -151,16 +160,16 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     line.upto = reinterpret_cast<unsigned*>(line.p0 + b.n + 1);
     int* status = parts.status;
 
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
         for (int i = 0; i < KS_STAGES; i++) {
             mbar_init(&bars.k_full[i], 4);
-            mbar_init(&bars.k_free[i], 1);
+            mbar_init(&bars.k_free[i], 2);
             mbar_init(&bars.v_full[i], 4);
-            mbar_init(&bars.v_free[i], 1);
+            mbar_init(&bars.v_free[i], 2);
         }
         for (int i = 0; i < 2; i++) {
             for (int j = 0; j < 2; j++) {
@@ -168,10 +177,10 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 mbar_init(&bars.p_full[i][j], 4);
             }
             mbar_init(&bars.o_done[i], 1);
+            mbar_init(&bars.all_done[i], 1);
         }
         mbar_init(&bars.q_full, 8);
-        mbar_init(&bars.unit_done, 1);
-        mbar_init(&bars.all_done, 1);
+        mbar_init(&bars.unit_done, 2);
         mbar_init_fence();
     }
     grid_wait();
@@ -192,7 +201,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         __syncthreads();
         all = 0;
 #pragma unroll
-        for (int w = 0; w < 13; w++) {
+        for (int w = 0; w < KS_WARPS; w++) {
             at += w < warp ? sh_scan[w] : 0;
             all += sh_scan[w];
         }
@@ -221,7 +230,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         if (lane == 0) before = 0;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 13; w++) before = max(before, w < warp ? (int)sh_scan[w] : 0);
+        for (int w = 0; w < KS_WARPS; w++) before = max(before, w < warp ? (int)sh_scan[w] : 0);
         for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) line.start[e] = before = max(before, line.start[e]);
         __syncthreads();
     }
@@ -306,9 +315,9 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         return s;
     };
 
-    if (begin >= end && tid == 0) parts.unit[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (warp < 8 && begin < end) {
+    if (warp < 8) {
         /* ================= softmax ================= */
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int x = warp >> 2, r = tid & 127; /* row tile, row */
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_o = tmem + (uint32_t)(x * 128) + lanes, t_s = tmem + 256u + (uint32_t)(x * 128) + lanes;
@@ -323,20 +332,20 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             const size_t at = ((size_t)(s.row0 + my_row) * cache.q_heads + my_head) * 128;
             float f = 0.0f;
             {
-                uint4 raw[16];
-#pragma unroll
-                for (int u = 0; u < 16; u++) raw[u] = live ? reinterpret_cast<const uint4*>(q + at)[u] : make_uint4(0, 0, 0, 0);
+                const uint4* from = reinterpret_cast<const uint4*>(q + (live ? at : 0)); /* (read twice, so that a row need not be held in registers) */
                 float big = 0.0f;
+#pragma unroll 8
+                for (int u = 0; u < 16; u++) {
+                    const uint4 w = live ? from[u] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int u = 0; u < 16; u++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) big = fmaxf(big, fmaxf(fabsf(bf_lo(ks_word(raw[u], i))), fabsf(bf_hi(ks_word(raw[u], i)))));
+                    for (int i = 0; i < 4; i++) big = fmaxf(big, fmaxf(fabsf(bf_lo(ks_word(w, i))), fabsf(bf_hi(ks_word(w, i)))));
+                }
                 const int e = big > 0.0f ? min(136 - (int)(__float_as_uint(big) >> 23), 120) : 0; /* 2^9 <= big 2^e < 2^10 */
                 const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                 f = __uint_as_float((uint32_t)(127 - e) << 23) * (1.4426950408889634f * 0.08838834764831845f); /* to base-2 logits: log2(e) / sqrt(128) */
-#pragma unroll
+#pragma unroll 8
                 for (int u = 0; u < 16; u++) { /* channels 0, 4, 1, 5, 2, 6, 3, 7 of the unit, as ks_widen puts them */
-                    const uint4 w = raw[u];
+                    const uint4 w = live ? from[u] : make_uint4(0, 0, 0, 0);
                     uint4 h;
                     h.x = ks_half2(bf_lo(w.x) * up, bf_lo(w.z) * up);
                     h.y = ks_half2(bf_hi(w.x) * up, bf_hi(w.z) * up);
@@ -462,38 +471,42 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             begun |= s.t0 == 0 && !whole;
             cur += (unsigned)(s.t1 - s.t0);
         }
-        if (tid == 0 && !begun) parts.unit[worker] = make_int4(0, 0, 0, 0);
-    } else if (warp >= 8 && warp < 12) {
+        if (tid == 0 && !begun) parts.unit[blockIdx.x] = make_int4(0, 0, 0, 0);
+    } else if (warp >= 8 && warp < 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         /* ================= pages to operands ================= */
-        const int p = tid - KS_SOFTMAX, g = lane >> 2, t = lane & 3, plane = (p >> 5) & 1;
+        const int team = (warp - 8) >> 2, p = tid & 127, g = lane >> 2, t = lane & 3, plane = (p >> 5) & 1;
         bool ok = true;
-        /* what to bring: its own walk along the stretch, KS_RAW - 1 pages ahead of the conversion */
+        /* what to bring: its own walk along the stretch, one page of the team ahead of the conversion */
         unsigned f_cur = begin, f_it = 0;
         int f_chunk = chunk_at, f_i = 0, page_of = -1; /* lane i keeps the (32 n + i)-th page of the segment */
         Segment f;
         f.t0 = f.t1 = 0;
-        auto bring = [&]() {
-            if (f_i == f.t1 - f.t0 && f_cur < end) {
-                f = segment(f_cur, f_chunk);
-                f_cur += (unsigned)(f.t1 - f.t0);
-                f_i = 0;
-            }
-            if (f_i < f.t1 - f.t0) {
+        auto bring = [&]() { /* the team's next page */
+            for (;;) {
+                if (f_i == f.t1 - f.t0) {
+                    if (f_cur == end) break;
+                    f = segment(f_cur, f_chunk);
+                    f_cur += (unsigned)(f.t1 - f.t0);
+                    f_i = 0;
+                }
                 if ((f_i & 31) == 0) {
                     const int pos = (f.t0 + f_i + lane) * S2P_B200_KV4_PAGE;
                     page_of = f_i + lane < f.t1 - f.t0 && pos < f.seen ? kv4_page(cache, f.seq, pos) : -1;
                 }
                 const int page = __shfl_sync(S2P_FULL_MASK, page_of, f_i & 31);
+                const unsigned now = f_it++;
+                f_i++;
+                if ((int)(now & 1) != team) continue;
                 if (page >= 0) {
                     const unsigned char* src = kv4_block(cache, page, f.head, 0) + p * 16;
-                    const uint32_t dst = smem_u32(raw) + f_it % KS_RAW * KV4_HEAD_BYTES + p * 16;
+                    const uint32_t dst = smem_u32(raw) + (team * KS_RAW + now / 2 % KS_RAW) * KV4_HEAD_BYTES + p * 16;
 #pragma unroll
                     for (int k = 0; k < KV4_HEAD_BYTES / 2048; k++)
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 2048), "l"(src + k * 2048) : "memory");
                 }
-                if (p == 0) sh_absent[f_it & 15] = page < 0;
-                f_i++;
-                f_it++;
+                if (p == 0) sh_absent[now & 15] = page < 0;
+                break;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -503,12 +516,13 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         for (unsigned cur = begin; cur < end && ok;) {
             const Segment s = segment(cur, chunk);
             for (int i = s.t0; i < s.t1; i++, it++) {
+                if ((int)(it & 1) != team) continue;
                 const unsigned stage = it % KS_STAGES, turn = it / KS_STAGES; /* the turn-th use of the stage */
                 asm volatile("cp.async.wait_group %0;" ::"n"(KS_RAW - 2) : "memory");
-                ks_pages_sync(); /* everybody's share of this page has come, and everybody is done with the one before it: */
+                ks_pages_sync(team); /* everybody's share of this page has come, and everybody is done with the one before it: */
                 bring();         /* ... its place is free */
                 const bool absent = *reinterpret_cast<volatile int*>(&sh_absent[it & 15]) != 0;
-                const unsigned char* page = raw + it % KS_RAW * KV4_HEAD_BYTES;
+                const unsigned char* page = raw + (team * KS_RAW + it / 2 % KS_RAW) * KV4_HEAD_BYTES;
                 /* a wait that has given up once is not waited for again, but the barriers above need every warp */
                 ok = ok && (turn == 0 || ks_wait_warp(&bars.k_free[stage], (turn - 1) & 1, status));
                 unsigned char* to = sk + stage * KS_K_BYTES;
@@ -558,93 +572,84 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             cur += (unsigned)(s.t1 - s.t0);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (begin < end) {
+    } else if (warp >= 16) {
         /* ================= the products ================= */
-        if (warp_elect()) {
-            /* D f32, A and B f16, M 128, N 64 and 128; B of the second product has its rows (positions) along K: MN-major */
-            const uint32_t idesc = (1u << 4) | (8u << 17) | (8u << 24), idesc_v = (1u << 4) | (16u << 17) | (8u << 24) | (1u << 16);
-            const uint64_t dq = ks_desc(smem_u32(sq), 2048, 128), dk = ks_desc(smem_u32(sk), KS_K_PITCH, 128);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        /* D f32, A and B f16, M 128, N 64 and 128; B of the second product has its rows (positions) along K: MN-major */
+        const uint32_t idesc = (1u << 4) | (8u << 17) | (8u << 24), idesc_v = (1u << 4) | (16u << 17) | (8u << 24) | (1u << 16);
+        /* A warp for each row tile, with a copy of the code each: with the tile as a variable the compiler keeps what the products take in ordinary
+         * registers and needs twice their time to issue them; and one warp for both waits for the one tile's weights while the other's are
+         * ready (1.4 us a page, the products 0.7). */
+        auto issue = [&](auto tile) {
+            constexpr int x = decltype(tile)::value;
+            const uint64_t dq = ks_desc(smem_u32(sq) + x * KS_Q_BYTES, 2048, 128), dk = ks_desc(smem_u32(sk), KS_K_PITCH, 128);
             const uint64_t dv = ks_desc(smem_u32(sv), 128, KS_V_PITCH);
-            unsigned stage = 0, turn = 0, n0 = 0, n1 = 0, segments = 0; /* n0, n1: pages of each row tile whose values have been asked for */
+            unsigned stage = 0, turn = 0, n = 0, segments = 0; /* n: pages whose values have been asked for */
             bool ok = true;
             int chunk = chunk_at;
-            /* Both row tiles are written out: with the tile as a loop's variable the compiler kept what the products take in ordinary registers, and a
-             * page's 24 products took 1.6 us to issue (their rate is 0.7). */
-            auto scores = [&](auto tile, unsigned page, unsigned from) {
-                constexpr int x = decltype(tile)::value;
-                const uint32_t d = tmem + 256u + x * 128 + 64u * (page & 1);
+            auto place = [&](unsigned page) { return tmem + 256u + x * 128 + 64u * (page & 1); };
+            auto scores = [&](unsigned page, unsigned from) {
+                const uint32_t d = place(page);
                 const uint64_t keys = dk + (uint64_t)(from * (KS_K_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < 8; k++) ks_mma_ss(d, dq + (uint64_t)((x * KS_Q_BYTES + k * 2 * 2048) >> 4), keys + (uint64_t)((k * 2 * KS_K_PITCH) >> 4), idesc, k > 0);
+                for (int k = 0; k < 8; k++) ks_mma_ss(d, dq + (uint64_t)((k * 2 * 2048) >> 4), keys + (uint64_t)((k * 2 * KS_K_PITCH) >> 4), idesc, k > 0);
                 ks_commit(&bars.s_full[x][page & 1]);
+                ks_commit(&bars.k_free[from]);
             };
-            auto values = [&](auto tile, unsigned page, bool add) {
-                constexpr int x = decltype(tile)::value;
-                const uint32_t d = tmem + 256u + x * 128 + 64u * (page & 1);
-                const uint64_t from = dv + (uint64_t)(stage * (KS_V_BYTES >> 4));
-#pragma unroll
-                for (int k = 0; k < 4; k++) ks_mma_ts(tmem + x * 128, d + 8 * k, from + (uint64_t)((k * 256) >> 4), idesc_v, add || k > 0);
-                ks_commit(&bars.o_done[x]);
-            };
-            const KsTile<0> first_tile;
-            const KsTile<1> second_tile;
             for (unsigned cur = begin; cur < end && ok; segments++) {
                 const Segment s = segment(cur, chunk);
                 const int tiles = s.t1 - s.t0;
-                const bool two = s.n_rows > tile_rows;
+                const bool active = s.n_rows > x * tile_rows;
                 ok = ks_wait(&bars.q_full, segments & 1, status) && ks_wait(&bars.k_full[stage], turn & 1, status);
                 if (!ok) break;
                 ks_after_sync();
-                scores(first_tile, n0, stage);
-                if (two) scores(second_tile, n1, stage);
-                ks_commit(&bars.k_free[stage]);
+                if (active) scores(n, stage);
+                else mbar_arrive(&bars.k_free[stage]);
                 for (int i = 0; i < tiles; i++) {
                     const unsigned next = stage + 1 == KS_STAGES ? 0 : stage + 1, next_turn = turn + (stage + 1 == KS_STAGES);
                     if (i + 1 < tiles) { /* the next scores take the place of the weights before these */
                         ok = ks_wait(&bars.k_full[next], next_turn & 1, status);
-                        if (ok && i > 0) ok = ks_wait(&bars.o_done[0], (n0 - 1) & 1, status);
+                        if (ok && active && i > 0) ok = ks_wait(&bars.o_done[x], (n - 1) & 1, status);
                         if (!ok) break;
                         ks_after_sync();
-                        scores(first_tile, n0 + 1, next);
-                        if (two) {
-                            if (i > 0) ok = ks_wait(&bars.o_done[1], (n1 - 1) & 1, status);
-                            if (!ok) break;
-                            ks_after_sync();
-                            scores(second_tile, n1 + 1, next);
-                        }
-                        ks_commit(&bars.k_free[next]);
+                        if (active) scores(n + 1, next);
+                        else mbar_arrive(&bars.k_free[next]);
                     }
-                    ok = ks_wait(&bars.v_full[stage], turn & 1, status) && ks_wait(&bars.p_full[0][n0 & 1], (n0 >> 1) & 1, status);
+                    ok = ks_wait(&bars.v_full[stage], turn & 1, status);
+                    if (ok && active) ok = ks_wait(&bars.p_full[x][n & 1], (n >> 1) & 1, status);
                     if (!ok) break;
                     ks_after_sync();
-                    values(first_tile, n0, i > 0);
-                    n0++;
-                    if (two) {
-                        ok = ks_wait(&bars.p_full[1][n1 & 1], (n1 >> 1) & 1, status);
-                        if (!ok) break;
-                        ks_after_sync();
-                        values(second_tile, n1, i > 0);
-                        n1++;
-                    }
-                    ks_commit(&bars.v_free[stage]);
+                    if (active) {
+                        const uint32_t d = place(n);
+                        const uint64_t from = dv + (uint64_t)(stage * (KS_V_BYTES >> 4));
+#pragma unroll
+                        for (int k = 0; k < 4; k++) ks_mma_ts(tmem + x * 128, d + 8 * k, from + (uint64_t)((k * 256) >> 4), idesc_v, i > 0 || k > 0);
+                        ks_commit(&bars.o_done[x]);
+                        ks_commit(&bars.v_free[stage]);
+                        n++;
+                    } else mbar_arrive(&bars.v_free[stage]);
                     stage = next;
                     turn = next_turn;
                 }
-                if (ok) ks_commit(&bars.unit_done);
+                if (ok) ks_commit(&bars.unit_done); /* (arrives at once where nothing is under way) */
                 cur += (unsigned)tiles;
             }
             /* TMEM must not be freed under products in flight: they complete by themselves, and this waits for them with a limit of its own */
-            ks_commit(&bars.all_done);
+            ks_commit(&bars.all_done[x]);
             PipeDeadline dl;
-            for (unsigned i = 0; i < PIPE_MBAR_TRIES && !mbar_try_wait(&bars.all_done, 0); i++)
+            for (unsigned i = 0; i < PIPE_MBAR_TRIES && !mbar_try_wait(&bars.all_done[x], 0); i++)
                 if ((i & 63u) == 63u && dl.expired(2000000000ull)) break;
+        };
+        if (begin < end && warp < 18 && warp_elect()) {
+            if (warp == 16) issue(KsTile<0>());
+            else issue(KsTile<1>());
         }
         __syncwarp();
     }
     ks_before_sync();
     __syncthreads();
     ks_after_sync();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 /* The parts of shared units, in order of the CTAs that left them.  Block (w, y): 16 rows of the unit that CTA w began; a thread has two units of
