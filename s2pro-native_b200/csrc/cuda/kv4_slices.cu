@@ -8,11 +8,11 @@
  *   O += P V     [128 x 128], P from TMEM, V in shared memory, f32 in TMEM
  *
  * Roles, coupled by mbarriers only:
- *   warps 0..3, 4..7   one thread a query row of the first, second tile: the row as f16 into shared memory (times a power of two, so that its
- *                      largest value is 512..1023: exact), then the softmax with the row's 64 scores in registers, at the end the result
+ *   warps 0..3, 4..7   one thread a query row of the first, second tile: the softmax with the row's 64 scores in registers, at the end the result
  *   warps 8..11, 12..15  every other page each: bring it into shared memory (with loads into registers, one page ahead, they waited for half their
  *                      time; one team of four warps alone took 1.4 us a page, twice what the products need) and turn it into operands: s c + m in f16 (one rounding, 2^-11), keys as [channel / 8][position] units of 8
- *                      channels, values likewise; three stages
+ *                      channels, values likewise; three stages.  A team also brings a row tile's queries, as f16 (times a power of two, so that
+ *                      a row's largest value is 512..1023: exact)
  *   warps 16, 17       one thread each issues a row tile's products.  Each row tile has two places for scores, so the scores of page i + 1 are
  *                      computed while the softmax of page i runs: it never waits for them.
  * Both row tiles use the same converted keys and values, which is what two of them are for.  Every operand is in the unswizzled
@@ -28,17 +28,17 @@
 namespace s2p {
 
 constexpr int KS_ROWS = 128, KS_TILE = S2P_B200_KV4_PAGE, KS_STAGES = 3, KS_RAW = 2, KS_WARPS = 20, KS_THREADS = KS_WARPS * 32, KS_SOFTMAX = 256;
-constexpr int KS_Q_BYTES = 16 * 128 * 16;                                  /* one row tile: [channel / 8][row] units */
+constexpr int KS_Q_PITCH = 128 * 16 + 16, KS_Q_BYTES = 16 * KS_Q_PITCH;                                  /* one row tile: [channel / 8][row] units */
 constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
 constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + 2 * KS_RAW * KV4_HEAD_BYTES;
-constexpr int KS_LEAST = 5;                                                /* pages that make a CTA worth its while */
+constexpr int KS_LEAST = 2;                                                /* pages that make a CTA worth its while */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
 struct KsBars {
     uint64_t k_full[KS_STAGES], k_free[KS_STAGES], v_full[KS_STAGES], v_free[KS_STAGES];
     uint64_t s_full[2][2], p_full[2][2]; /* [row tile][place] */
-    uint64_t o_done[2], q_full, unit_done, all_done[2];
+    uint64_t o_done[2], q_full, q_free, unit_done, all_done[2];
 };
 
 struct KsLine { /* in shared memory: the chunks (units of one kv head each) of all entries */
@@ -121,6 +121,24 @@ __device__ __forceinline__ float ks_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+/* two at a time; three at a time */
+__device__ __forceinline__ float2 ks_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 ks_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float ks_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ uint32_t ks_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -146,7 +164,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ KsBars bars;
     __shared__ uint32_t sh_tmem;
-    __shared__ unsigned sh_scan[KS_WARPS];
+    __shared__ float sh_factor[4][KS_SOFTMAX]; /* of the query rows of a unit, four units deep: to base-2 logits */
     __shared__ int sh_absent[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = cache.q_heads / cache.kv_heads, tile_rows = KS_ROWS / group, unit_rows = 2 * tile_rows;
@@ -180,6 +198,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             mbar_init(&bars.all_done[i], 1);
         }
         mbar_init(&bars.q_full, 8);
+        mbar_init(&bars.q_free, 2);
         mbar_init(&bars.unit_done, 2);
         mbar_init_fence();
     }
@@ -187,69 +206,9 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     grid_release();
     ks_before_sync();
 
-    /* ---- the line of work ---- */
-    auto block_scan = [&](unsigned v, unsigned& all) { /* sum over the threads before this one, and over all */
-        unsigned at = v;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
-            if (lane >= off) at += o;
-        }
-        __syncthreads();
-        if (lane == 31) sh_scan[warp] = at;
-        at -= v;
-        __syncthreads();
-        all = 0;
-#pragma unroll
-        for (int w = 0; w < KS_WARPS; w++) {
-            at += w < warp ? sh_scan[w] : 0;
-            all += sh_scan[w];
-        }
-        return at;
-    };
-    const int per = b.n / KS_THREADS + 1;
-    {
-        int top = 0; /* starts made ascending and kept inside the activations, whatever row0 holds */
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
-            const int r = b.row0[e];
-            if (e < b.n) {
-                const int seq = b.seqs[e], p0 = b.pos0[e];
-                line.seq[e] = seq;
-                line.p0[e] = (unsigned)seq < (unsigned)cache.max_seqs && p0 <= (1 << 30) ? p0 : -1;
-            }
-            top = max(top, line.start[e] = min(r, b.rows));
-        }
-        int before = top;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(S2P_FULL_MASK, before, off);
-            if (lane >= off) before = max(before, o);
-        }
-        if (lane == 31) sh_scan[warp] = (unsigned)before;
-        before = __shfl_up_sync(S2P_FULL_MASK, before, 1);
-        if (lane == 0) before = 0;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < KS_WARPS; w++) before = max(before, w < warp ? (int)sh_scan[w] : 0);
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) line.start[e] = before = max(before, line.start[e]);
-        __syncthreads();
-    }
-    ks_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh_tmem);
     auto rows_of = [&](int e) { return line.start[e + 1] - line.start[e]; };
     auto chunks_of = [&](int e) { return rows_of(e) > few ? (rows_of(e) + unit_rows - 1) / unit_rows : 0; };
     auto seen_by = [&](int p0, int row) { return p0 < 0 ? 0 : (int)min((long long)p0 + row + 1, (long long)capacity); };
-    unsigned chunks, total;
-    {
-        unsigned sum = 0;
-        for (int i = 0, e = tid * per; i < per && e < b.n; i++, e++) sum += (unsigned)chunks_of(e);
-        unsigned at = block_scan(sum, chunks);
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
-            line.first[e] = (int)at;
-            if (e < b.n) at += (unsigned)chunks_of(e);
-        }
-        __syncthreads();
-    }
     auto entry_of = [&](int chunk) { /* the entry whose chunk it is */
         int lo = 0, hi = b.n;
         while (hi - lo > 1) {
@@ -258,26 +217,59 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         }
         return lo;
     };
-    auto tiles_of = [&](int e, int chunk) { /* position tiles of a chunk's unit */
+    auto tiles_of = [&](int e, int chunk) { /* pages of a chunk's unit */
         const int last = min(rows_of(e), (chunk - line.first[e] + 1) * unit_rows) - 1;
         return max(1, (seen_by(line.p0[e], last) + KS_TILE - 1) / KS_TILE);
     };
-    {
-        const int each = (int)chunks / KS_THREADS + 1;
-        unsigned sum = 0;
-        for (int i = 0, c = tid * each; i < each && c < (int)chunks; i++, c++) {
-            const unsigned t = (unsigned)tiles_of(entry_of(c), c) * (unsigned)cache.kv_heads;
-            line.upto[c] = t;
-            sum += t;
+    /* ---- the line of work, by one warp: 32 entries or chunks at a time, so no barrier for the usual few ---- */
+    if (warp == 0) {
+        int top = 0; /* starts made ascending and kept inside the activations, whatever row0 holds */
+        for (int e0 = 0; e0 <= b.n; e0 += 32) {
+            const int e = e0 + lane;
+            int r = e <= b.n ? min(b.row0[e], b.rows) : 0;
+            if (e < b.n) {
+                const int seq = b.seqs[e], p0 = b.pos0[e];
+                line.seq[e] = seq;
+                line.p0[e] = (unsigned)seq < (unsigned)cache.max_seqs && p0 <= (1 << 30) ? p0 : -1;
+            }
+            r = max(r, top);
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(S2P_FULL_MASK, r, off);
+                if (lane >= off) r = max(r, o);
+            }
+            if (e <= b.n) line.start[e] = r;
+            top = __shfl_sync(S2P_FULL_MASK, r, 31);
         }
-        unsigned at = block_scan(sum, total);
-        for (int i = 0, c = tid * each; i < each && c <= (int)chunks; i++, c++) {
-            const unsigned t = c < (int)chunks ? line.upto[c] : 0;
-            line.upto[c] = at;
-            at += t;
+        __syncwarp();
+        auto before = [&](unsigned v, unsigned& carry) { /* carry + the lanes before this one; carry goes on */
+            unsigned at = v;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
+                if (lane >= off) at += o;
+            }
+            const unsigned all = __shfl_sync(S2P_FULL_MASK, at, 31), mine = carry + at - v;
+            carry += all;
+            return mine;
+        };
+        unsigned chunks = 0, total = 0;
+        for (int e0 = 0; e0 <= b.n; e0 += 32) {
+            const int e = e0 + lane;
+            const unsigned at = before(e < b.n ? (unsigned)chunks_of(e) : 0u, chunks);
+            if (e <= b.n) line.first[e] = (int)at;
         }
-        __syncthreads();
+        __syncwarp();
+        for (int c0 = 0; c0 <= (int)chunks; c0 += 32) {
+            const int c = c0 + lane;
+            const unsigned at = before(c < (int)chunks ? (unsigned)tiles_of(entry_of(c), c) * (unsigned)cache.kv_heads : 0u, total);
+            if (c <= (int)chunks) line.upto[c] = at;
+        }
     }
+    __syncthreads();
+    ks_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh_tmem);
+    const unsigned chunks = (unsigned)line.first[b.n], total = line.upto[chunks];
     const unsigned workers = min(gridDim.x, (total + KS_LEAST - 1) / KS_LEAST);
     const unsigned share = workers ? total / workers : 1, more = workers ? total - share * workers : 0, worker = blockIdx.x;
     const unsigned begin = worker < workers ? share * worker + min(worker, more) : 0, end = worker < workers ? begin + share + (worker < more) : 0;
@@ -315,6 +307,87 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         return s;
     };
 
+    const int team = (warp >> 2) & 1, p = tid & 127;
+            /* The teams of warps 8..11 and 12..15: what to bring, a walk along the stretch of its own along the stretch, one page of the team ahead of the conversion */
+            unsigned f_cur = begin, f_it = 0;
+            int f_chunk = chunk_at, f_i = 0, page_of = -1; /* lane i keeps the (32 n + i)-th page of the segment */
+            Segment f;
+            f.t0 = f.t1 = 0;
+            auto bring = [&]() { /* the team's next page */
+                for (;;) {
+                    if (f_i == f.t1 - f.t0) {
+                        if (f_cur == end) break;
+                        f = segment(f_cur, f_chunk);
+                        f_cur += (unsigned)(f.t1 - f.t0);
+                        f_i = 0;
+                    }
+                    if ((f_i & 31) == 0) {
+                        const int pos = (f.t0 + f_i + lane) * S2P_B200_KV4_PAGE;
+                        page_of = f_i + lane < f.t1 - f.t0 && pos < f.seen ? kv4_page(cache, f.seq, pos) : -1;
+                    }
+                    const int page = __shfl_sync(S2P_FULL_MASK, page_of, f_i & 31);
+                    const unsigned now = f_it++;
+                    f_i++;
+                    if ((int)(now & 1) != team) continue;
+                    if (page >= 0) {
+                        const unsigned char* src = kv4_block(cache, page, f.head, 0) + p * 16;
+                        const uint32_t dst = smem_u32(raw) + (team * KS_RAW + now / 2 % KS_RAW) * KV4_HEAD_BYTES + p * 16;
+    #pragma unroll
+                        for (int k = 0; k < KV4_HEAD_BYTES / 2048; k++)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 2048), "l"(src + k * 2048) : "memory");
+                    }
+                    if (p == 0) sh_absent[now & 15] = page < 0;
+                    break;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+    /* The query rows of a unit from row tile `tile`, a row to half a warp (a lane has 16 bytes of it), eight rows' loads under way; `first` and `step`:
+     * what rows are this half warp's. */
+    const unsigned by_group = (65536u + (unsigned)group - 1) / (unsigned)group; /* r / group = r by_group >> 16 for r < 128 */
+    auto queries = [&](const Segment& s, unsigned unit, int tile, int first, int step) {
+        if (s.n_rows <= tile * tile_rows) return;
+        const int u = lane & 15;
+        for (int r0 = first; r0 < KS_ROWS; r0 += 8 * step) {
+            uint4 w[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int r = r0 + k * step, in = (int)((unsigned)r * by_group >> 16), row = tile * tile_rows + in;
+                w[k] = make_uint4(0, 0, 0, 0);
+                if (in < tile_rows && row < s.n_rows && r < KS_ROWS)
+                    w[k] = reinterpret_cast<const uint4*>(q + ((size_t)(s.row0 + row) * cache.q_heads + (s.head * group + r - in * group)) * 128)[u];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int r = r0 + k * step;
+                /* the largest magnitude of the row, by the bits */
+                uint32_t big = __vmaxu2(__vmaxu2(w[k].x & 0x7FFF7FFFu, w[k].y & 0x7FFF7FFFu), __vmaxu2(w[k].z & 0x7FFF7FFFu, w[k].w & 0x7FFF7FFFu));
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1) big = __vmaxu2(big, __shfl_xor_sync(S2P_FULL_MASK, big, off));
+                const int largest = (int)max(big & 0xFFFFu, big >> 16), e = largest ? min(136 - (largest >> 7), 120) : 0; /* 2^9 <= it times 2^e < 2^10 */
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                if (r < KS_ROWS) {
+                    if (u == 0) /* log2(e) / sqrt(128) 2^-e */
+                        sh_factor[unit & 3][tile * KS_ROWS + r] = __uint_as_float((uint32_t)(127 - e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
+                    uint4 h; /* channels 0, 4, 1, 5, 2, 6, 3, 7 of the unit of eight, as ks_widen puts them */
+                    h.x = ks_half2(bf_lo(w[k].x) * up, bf_lo(w[k].z) * up);
+                    h.y = ks_half2(bf_hi(w[k].x) * up, bf_hi(w[k].z) * up);
+                    h.z = ks_half2(bf_lo(w[k].y) * up, bf_lo(w[k].w) * up);
+                    h.w = ks_half2(bf_hi(w[k].y) * up, bf_hi(w[k].w) * up);
+                    *reinterpret_cast<uint4*>(sq + tile * KS_Q_BYTES + u * KS_Q_PITCH + r * 16) = h;
+                }
+            }
+        }
+        fence_proxy_async_smem();
+    };
+    if (begin < end) {
+        if (warp >= 8 && warp < 16) /* the first pages are under way while everybody brings the first unit's queries */
+            for (int i = 0; i < KS_RAW - 1; i++) bring();
+        int chunk = chunk_at;
+        const Segment s = segment(begin, chunk);
+        if (warp < 16) queries(s, 0, warp >> 3, (warp & 7) * 2 + (lane >> 4), 16);
+    }
+    __syncthreads();
+
     if (warp < 8) {
         /* ================= softmax ================= */
         asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
@@ -330,34 +403,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             const int my_row = x * tile_rows + r / group, my_head = s.head * group + r % group;
             const bool live = r < tile_rows * group && my_row < s.n_rows, active = x * tile_rows < s.n_rows;
             const size_t at = ((size_t)(s.row0 + my_row) * cache.q_heads + my_head) * 128;
-            float f = 0.0f;
-            {
-                const uint4* from = reinterpret_cast<const uint4*>(q + (live ? at : 0)); /* (read twice, so that a row need not be held in registers) */
-                float big = 0.0f;
-#pragma unroll 8
-                for (int u = 0; u < 16; u++) {
-                    const uint4 w = live ? from[u] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) big = fmaxf(big, fmaxf(fabsf(bf_lo(ks_word(w, i))), fabsf(bf_hi(ks_word(w, i)))));
-                }
-                const int e = big > 0.0f ? min(136 - (int)(__float_as_uint(big) >> 23), 120) : 0; /* 2^9 <= big 2^e < 2^10 */
-                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-                f = __uint_as_float((uint32_t)(127 - e) << 23) * (1.4426950408889634f * 0.08838834764831845f); /* to base-2 logits: log2(e) / sqrt(128) */
-#pragma unroll 8
-                for (int u = 0; u < 16; u++) { /* channels 0, 4, 1, 5, 2, 6, 3, 7 of the unit, as ks_widen puts them */
-                    const uint4 w = live ? from[u] : make_uint4(0, 0, 0, 0);
-                    uint4 h;
-                    h.x = ks_half2(bf_lo(w.x) * up, bf_lo(w.z) * up);
-                    h.y = ks_half2(bf_hi(w.x) * up, bf_hi(w.z) * up);
-                    h.z = ks_half2(bf_lo(w.y) * up, bf_lo(w.w) * up);
-                    h.w = ks_half2(bf_hi(w.y) * up, bf_hi(w.w) * up);
-                    *reinterpret_cast<uint4*>(sq + x * KS_Q_BYTES + (u * 128 + r) * 16) = h;
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.q_full);
-
+            float f = 0.0f; /* (there with the first scores, which were issued behind it) */
             const int limit = live ? seen_by(s.p0, s.r0 + my_row) : s.seen;
             float top = -INFINITY, sum = 0.0f;
             if (active)
@@ -366,6 +412,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     ok = ks_wait_warp(&bars.s_full[x][place], (n_s >> 1) & 1, status);
                     if (!ok) break;
                     ks_after_sync();
+                    if (i == s.t0) f = *reinterpret_cast<volatile float*>(&sh_factor[segments & 3][tid]);
                     uint32_t v[2][32];
                     ks_ld32(t_s + 64 * place, v[0]);
                     ks_ld32(t_s + 64 * place + 32, v[1]);
@@ -378,8 +425,8 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     }
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int k = 0; k < 64; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k >> 5][k & 31]));
-                    const float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+                    for (int k = 0; k < 64; k += 2) m4[(k >> 1) & 3] = ks_max3(m4[(k >> 1) & 3], __uint_as_float(v[k >> 5][k & 31]), __uint_as_float(v[k >> 5][(k + 1) & 31]));
+                    const float most = ks_max3(ks_max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * f;
                     if (__any_sync(S2P_FULL_MASK, most > top + 8.0f)) {
                         const float now = fmaxf(most, top), shrink = now == -INFINITY ? 1.0f : ks_exp2(top - now);
                         top = now;
@@ -400,19 +447,23 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                         }
                     }
                     const float base = top == -INFINITY ? 0.0f : top;
-                    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const float2 f2 = make_float2(f, f), minus = make_float2(-base, -base);
+                    float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         uint32_t p[16];
 #pragma unroll
                         for (int k = 0; k < 16; k++) {
-                            const float a = ks_exp2(fmaf(__uint_as_float(v[h][2 * k]), f, -base)), d = ks_exp2(fmaf(__uint_as_float(v[h][2 * k + 1]), f, -base));
-                            s4[k & 3] += a + d;
-                            p[k] = ks_half2(a, d);
+                            const float2 a = ks_fma2(make_float2(__uint_as_float(v[h][2 * k]), __uint_as_float(v[h][2 * k + 1])), f2, minus);
+                            const float2 w = make_float2(ks_exp2(a.x), ks_exp2(a.y));
+                            s2[k & 1] = ks_add2(s2[k & 1], w);
+                            p[k] = ks_half2(w.x, w.y);
                         }
                         ks_st16(t_s + 64 * place + 16 * h, p); /* over scores that are in registers */
                     }
-                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    if (!ok) break;
+                    const float2 both = ks_add2(s2[0], s2[1]);
+                    sum += both.x + both.y;
                     ks_st_wait();
                     ks_before_sync();
                     __syncwarp();
@@ -475,46 +526,24 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     } else if (warp >= 8 && warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         /* ================= pages to operands ================= */
-        const int team = (warp - 8) >> 2, p = tid & 127, g = lane >> 2, t = lane & 3, plane = (p >> 5) & 1;
+        const int g = lane >> 2, t = lane & 3, plane = (p >> 5) & 1;
         bool ok = true;
-        /* what to bring: its own walk along the stretch, one page of the team ahead of the conversion */
-        unsigned f_cur = begin, f_it = 0;
-        int f_chunk = chunk_at, f_i = 0, page_of = -1; /* lane i keeps the (32 n + i)-th page of the segment */
-        Segment f;
-        f.t0 = f.t1 = 0;
-        auto bring = [&]() { /* the team's next page */
-            for (;;) {
-                if (f_i == f.t1 - f.t0) {
-                    if (f_cur == end) break;
-                    f = segment(f_cur, f_chunk);
-                    f_cur += (unsigned)(f.t1 - f.t0);
-                    f_i = 0;
-                }
-                if ((f_i & 31) == 0) {
-                    const int pos = (f.t0 + f_i + lane) * S2P_B200_KV4_PAGE;
-                    page_of = f_i + lane < f.t1 - f.t0 && pos < f.seen ? kv4_page(cache, f.seq, pos) : -1;
-                }
-                const int page = __shfl_sync(S2P_FULL_MASK, page_of, f_i & 31);
-                const unsigned now = f_it++;
-                f_i++;
-                if ((int)(now & 1) != team) continue;
-                if (page >= 0) {
-                    const unsigned char* src = kv4_block(cache, page, f.head, 0) + p * 16;
-                    const uint32_t dst = smem_u32(raw) + (team * KS_RAW + now / 2 % KS_RAW) * KV4_HEAD_BYTES + p * 16;
-#pragma unroll
-                    for (int k = 0; k < KV4_HEAD_BYTES / 2048; k++)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 2048), "l"(src + k * 2048) : "memory");
-                }
-                if (p == 0) sh_absent[now & 15] = page < 0;
-                break;
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        for (int i = 0; i < KS_RAW - 1; i++) bring();
-        unsigned it = 0;
+        unsigned it = 0, segments = 0;
         int chunk = chunk_at;
-        for (unsigned cur = begin; cur < end && ok;) {
+        for (unsigned cur = begin; cur < end && ok; segments++) {
             const Segment s = segment(cur, chunk);
+            /* The queries of a unit go where the unit's before were as soon as its last scores are complete, while its last softmax and its result
+             * are still to come; behind the team's first page of the unit, which waits for less. */
+            bool have_q = segments == 0;
+            auto next_queries = [&]() {
+                ok = ok && ks_wait_warp(&bars.q_free, (segments - 1) & 1, status);
+                if (ok) {
+                    queries(s, segments, team, (warp & 3) * 2 + (lane >> 4), 8);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.q_full);
+                }
+                have_q = true;
+            };
             for (int i = s.t0; i < s.t1; i++, it++) {
                 if ((int)(it & 1) != team) continue;
                 const unsigned stage = it % KS_STAGES, turn = it / KS_STAGES; /* the turn-th use of the stage */
@@ -568,7 +597,9 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.v_full[stage]);
                 }
+                if (!have_q) next_queries();
             }
+            if (!have_q) next_queries();
             cur += (unsigned)(s.t1 - s.t0);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -582,7 +613,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
          * ready (1.4 us a page, the products 0.7). */
         auto issue = [&](auto tile) {
             constexpr int x = decltype(tile)::value;
-            const uint64_t dq = ks_desc(smem_u32(sq) + x * KS_Q_BYTES, 2048, 128), dk = ks_desc(smem_u32(sk), KS_K_PITCH, 128);
+            const uint64_t dq = ks_desc(smem_u32(sq) + x * KS_Q_BYTES, KS_Q_PITCH, 128), dk = ks_desc(smem_u32(sk), KS_K_PITCH, 128);
             const uint64_t dv = ks_desc(smem_u32(sv), 128, KS_V_PITCH);
             unsigned stage = 0, turn = 0, n = 0, segments = 0; /* n: pages whose values have been asked for */
             bool ok = true;
@@ -592,7 +623,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 const uint32_t d = place(page);
                 const uint64_t keys = dk + (uint64_t)(from * (KS_K_BYTES >> 4));
 #pragma unroll
-                for (int k = 0; k < 8; k++) ks_mma_ss(d, dq + (uint64_t)((k * 2 * 2048) >> 4), keys + (uint64_t)((k * 2 * KS_K_PITCH) >> 4), idesc, k > 0);
+                for (int k = 0; k < 8; k++) ks_mma_ss(d, dq + (uint64_t)((k * 2 * KS_Q_PITCH) >> 4), keys + (uint64_t)((k * 2 * KS_K_PITCH) >> 4), idesc, k > 0);
                 ks_commit(&bars.s_full[x][page & 1]);
                 ks_commit(&bars.k_free[from]);
             };
@@ -600,20 +631,25 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 const Segment s = segment(cur, chunk);
                 const int tiles = s.t1 - s.t0;
                 const bool active = s.n_rows > x * tile_rows;
-                ok = ks_wait(&bars.q_full, segments & 1, status) && ks_wait(&bars.k_full[stage], turn & 1, status);
+                ok = (segments == 0 || ks_wait(&bars.q_full, (segments - 1) & 1, status)) && ks_wait(&bars.k_full[stage], turn & 1, status);
                 if (!ok) break;
                 ks_after_sync();
                 if (active) scores(n, stage);
                 else mbar_arrive(&bars.k_free[stage]);
+                if (tiles == 1) ks_commit(&bars.q_free);
                 for (int i = 0; i < tiles; i++) {
                     const unsigned next = stage + 1 == KS_STAGES ? 0 : stage + 1, next_turn = turn + (stage + 1 == KS_STAGES);
-                    if (i + 1 < tiles) { /* the next scores take the place of the weights before these */
+                    /* The next scores, of this unit or of the one behind it, take the place of the weights before these: that product has to be
+                     * complete.  (Waited for at every page, or this would fall two phases behind.) */
+                    if (active && n >= 1) ok = ks_wait(&bars.o_done[x], (n - 1) & 1, status);
+                    if (!ok) break;
+                    if (i + 1 < tiles) {
                         ok = ks_wait(&bars.k_full[next], next_turn & 1, status);
-                        if (ok && active && i > 0) ok = ks_wait(&bars.o_done[x], (n - 1) & 1, status);
                         if (!ok) break;
                         ks_after_sync();
                         if (active) scores(n + 1, next);
                         else mbar_arrive(&bars.k_free[next]);
+                        if (i + 2 == tiles) ks_commit(&bars.q_free); /* (arrives at once where nothing is under way) */
                     }
                     ok = ks_wait(&bars.v_full[stage], turn & 1, status);
                     if (ok && active) ok = ks_wait(&bars.p_full[x][n & 1], (n >> 1) & 1, status);
@@ -631,7 +667,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     stage = next;
                     turn = next_turn;
                 }
-                if (ok) ks_commit(&bars.unit_done); /* (arrives at once where nothing is under way) */
+                if (ok) ks_commit(&bars.unit_done);
                 cur += (unsigned)tiles;
             }
             /* TMEM must not be freed under products in flight: they complete by themselves, and this waits for them with a limit of its own */
@@ -715,7 +751,7 @@ static int ks_chunks(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b) {
     const long long most = (long long)b->rows / unit + (b->n < b->rows ? b->n : b->rows);
     return most < (1 << 20) ? (int)most : 1 << 20;
 }
-constexpr int KS_MOST_SMEM = 225 * 1024;
+constexpr int KS_MOST_SMEM = 221 * 1024; /* 227 KB less what is declared in the kernel */
 
 extern "C" int kv4_slices_serve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b) {
     return KS_OPERANDS + ks_line_bytes(ks_chunks(c, b), b->n) <= (size_t)KS_MOST_SMEM;
