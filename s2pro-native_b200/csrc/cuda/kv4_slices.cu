@@ -506,14 +506,14 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     for (int k = 0; k < 32; k++) y[k] = __uint_as_float(v[k]);
                     if (whole) {
                         if (live) store(c, y, sum == 0.0f ? 0.0f : 1.0f / sum);
-                    } else {
+                    } else if (live) {
 #pragma unroll
                         for (int k = 0; k < 8; k++)
                             parts.o[(slot * 32 + 8 * c + k) * KS_SOFTMAX + tid] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
                     }
                 }
                 ks_before_sync(); /* the next unit's first product writes where this has been read */
-                if (!whole) {
+                if (!whole && live) {
                     parts.max[slot * KS_SOFTMAX + tid] = top;
                     parts.sum[slot * KS_SOFTMAX + tid] = sum;
                 }
@@ -688,43 +688,48 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-/* The parts of shared units, in order of the CTAs that left them.  Block (w, y): 16 rows of the unit that CTA w began; a thread has two units of
- * channels of a row, and four parts' loads are under way at a time. */
-constexpr int KS_JOIN_ROWS = 16, KS_JOIN_THREADS = 128;
+/* The parts of shared units, in order of the CTAs that left them.  Block (w, y): 32 rows of the unit that CTA w began; a thread has one unit of eight
+ * columns of a row, and eight parts' loads are under way at a time. */
+constexpr int KS_JOIN_ROWS = 32, KS_JOIN_THREADS = 16 * KS_JOIN_ROWS, KS_JOIN_PARTS = 8;
 __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int q_heads, int group, __nv_bfloat16* out) {
     grid_wait();
     grid_release();
-    const int w0 = blockIdx.x, r = blockIdx.y * KS_JOIN_ROWS + (threadIdx.x & 15), u = threadIdx.x >> 4;
+    const int w0 = blockIdx.x, r = blockIdx.y * KS_JOIN_ROWS + (threadIdx.x % KS_JOIN_ROWS), u = threadIdx.x / KS_JOIN_ROWS;
     const int4 unit = parts.unit[w0];
     const int tile_rows = KS_ROWS / group, x = r / KS_ROWS, in = r % KS_ROWS, row = x * tile_rows + in / group;
     if (in >= tile_rows * group || row >= unit.y) return;
     const int w1 = unit.w;
-    float top = -INFINITY, sum = 0.0f, y[16];
+    float top = -INFINITY, sum = 0.0f, y[8];
 #pragma unroll
-    for (int k = 0; k < 16; k++) y[k] = 0.0f;
-    for (int w = w0; w <= w1; w += 4) {
-        float m[4], l[4];
-        float4 v[4][4];
+    for (int k = 0; k < 8; k++) y[k] = 0.0f;
+    for (int w = w0; w <= w1; w += KS_JOIN_PARTS) {
+        float m[KS_JOIN_PARTS], l[KS_JOIN_PARTS];
+        float4 v[KS_JOIN_PARTS][2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool there = w + i <= w1;
-            const size_t slot = (size_t)(2 * (w + i) + (w + i == w0));
-            m[i] = there ? __ldcg(parts.max + slot * KS_SOFTMAX + r) : -INFINITY;
-            l[i] = there ? __ldcg(parts.sum + slot * KS_SOFTMAX + r) : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) /* units u and u + 8 */
-                v[i][k] = there ? __ldcg(parts.o + (slot * 32 + 2 * u + (k & 1) + 16 * (k >> 1)) * KS_SOFTMAX + r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = 0; i < KS_JOIN_PARTS; i++) { /* (past the last part: its own again, with no weight) */
+            const int at = min(w + i, w1);
+            const size_t slot = (size_t)(2 * at + (at == w0));
+            m[i] = __ldcg(parts.max + slot * KS_SOFTMAX + r);
+            l[i] = __ldcg(parts.sum + slot * KS_SOFTMAX + r);
+            v[i][0] = __ldcg(parts.o + (slot * 32 + 2 * u) * KS_SOFTMAX + r);
+            v[i][1] = __ldcg(parts.o + (slot * 32 + 2 * u + 1) * KS_SOFTMAX + r);
         }
-        const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), base = now == -INFINITY ? 0.0f : now, keep = ks_exp2(top - base);
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < KS_JOIN_PARTS; i++) {
+            if (w + i > w1) m[i] = -INFINITY;
+            now = fmaxf(now, m[i]);
+        }
+        const float base = now == -INFINITY ? 0.0f : now, keep = ks_exp2(top - base);
         sum *= keep;
 #pragma unroll
-        for (int k = 0; k < 16; k++) y[k] *= keep;
+        for (int k = 0; k < 8; k++) y[k] *= keep;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < KS_JOIN_PARTS; i++) {
             const float scale = ks_exp2(m[i] - base);
             sum = fmaf(l[i], scale, sum);
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < 2; k++) {
                 y[4 * k] = fmaf(v[i][k].x, scale, y[4 * k]);
                 y[4 * k + 1] = fmaf(v[i][k].y, scale, y[4 * k + 1]);
                 y[4 * k + 2] = fmaf(v[i][k].z, scale, y[4 * k + 2]);
@@ -734,15 +739,12 @@ __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int
         top = now;
     }
     const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-    __nv_bfloat16* to = out + ((size_t)(unit.x + row) * q_heads + unit.z * group + in % group) * 128 + 4 * u;
+    __nv_bfloat16* to = out + ((size_t)(unit.x + row) * q_heads + unit.z * group + in % group) * 128 + 64 * (u >> 3) + 4 * (u & 7);
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int odd = 0; odd < 2; odd++) {
-            const __nv_bfloat162 a = __floats2bfloat162_rn(y[8 * h + odd] * scale, y[8 * h + 2 + odd] * scale),
-                                 d = __floats2bfloat162_rn(y[8 * h + 4 + odd] * scale, y[8 * h + 6 + odd] * scale);
-            *reinterpret_cast<uint2*>(to + 64 * h + 32 * odd) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&d));
-        }
+    for (int odd = 0; odd < 2; odd++) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(y[odd] * scale, y[2 + odd] * scale), d = __floats2bfloat162_rn(y[4 + odd] * scale, y[6 + odd] * scale);
+        *reinterpret_cast<uint2*>(to + 32 * odd) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&d));
+    }
 }
 
 /* chunks that the batch can have: its rows in units, and a broken one for each entry */
