@@ -56,37 +56,50 @@ __device__ __forceinline__ bool kv4_find(const Kv4View& v, const Kv4Rows& b, int
     return true;
 }
 
-/* Byte offset, inside a block, of the two bytes that hold channels 4 l .. 4 l + 3 (lane l's) of position i */
-__device__ __forceinline__ int kv4_key_at(int i, int l) { return 64 * i + 16 * ((l & 7) >> 1) + 4 * (l >> 3) + 2 * (l & 1); }
-__device__ __forceinline__ int kv4_value_at(int i, int l) {
-    return 1024 + 512 * (i >> 3) + 64 * (l & 7) + 16 * ((i >> 1) & 3) + 8 * (i & 1) + 2 * (l >> 3);
-}
+/* A head vector in half a warp: lane l (0 .. 15) has channels 8 l .. 8 l + 7, four lanes a group.  Byte offsets, inside a block, of what the
+ * lane has of position i: the four bytes of a key; the two bytes of the first four channels of a value, those of the others 64 on; */
+__device__ __forceinline__ int kv4_key_at(int i, int l) { return 64 * i + 16 * (l & 3) + 4 * (l >> 2); }
+__device__ __forceinline__ int kv4_value_at(int i, int l) { return 1024 + 512 * (i >> 3) + 128 * (l & 3) + 16 * ((i >> 1) & 3) + 8 * (i & 1) + 2 * (l >> 2); }
 /* ... and of s of group j of position i; m of a key 8 bytes on, of a value 128 */
 __device__ __forceinline__ int kv4_key_param_at(int i, int j) { return KV4_PARAMS_K + 16 * i + 2 * j; }
 __device__ __forceinline__ int kv4_value_param_at(int i, int j) { return KV4_PARAMS_V + 16 * (i >> 1) + 4 * j + 2 * (i & 1); }
 
-/* A head vector in a warp, four channels a lane, eight lanes a group: the lane's codes (low four bits the first channel) and
- * its group's s and m.  fminf and fmaxf pass over a NaN, and its code comes out of the conversion as 0. */
-__device__ __forceinline__ uint32_t kv4_quantise(const float x[4], __half& s_out, __half& m_out) {
-    float v[4];
+/* The lane's codes (low four bits the first channel) and its group's s and m.  `half`: the lanes of the half warp.  fminf and fmaxf pass over
+ * a NaN, and clamping it makes it the least. */
+__device__ __forceinline__ uint32_t kv4_quantise(float (&v)[8], unsigned half, __half& s_out, __half& m_out) {
+    bool fits = true;
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = x[i] != x[i] ? x[i] : fminf(fmaxf(x[i], -65504.0f), 65504.0f);
-    float lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    for (int i = 0; i < 8; i++) fits = fits && fabsf(v[i]) <= 65504.0f;
+    if (!fits)
 #pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(S2P_FULL_MASK, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(S2P_FULL_MASK, hi, off));
+        for (int i = 0; i < 8; i++) v[i] = v[i] != v[i] ? v[i] : fminf(fmaxf(v[i], -65504.0f), 65504.0f);
+    float lo = fminf(fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), fminf(fminf(v[4], v[5]), fminf(v[6], v[7])));
+    float hi = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(half, lo, off));
+        hi = fmaxf(hi, __shfl_xor_sync(half, hi, off));
     }
     if (!(lo <= hi)) lo = hi = 0.0f; /* nothing but NaN */
     s_out = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
     m_out = __float2half_rn(lo);
-    const float s = __half2float(s_out), m = __half2float(m_out);
+    const float s = __half2float(s_out), m = __half2float(m_out), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    /* To the nearest whole number, ties to even, by adding 2^23 + 2^22, which leaves it in the low bits.  A quotient by way of the reciprocal is off by
+     * less than 1e-5 (it is at most 16 and a bit, three roundings), so it rounds to the same code unless it lies that close to the middle
+     * between two: then it is divided after all. */
+    const float big = 12582912.0f;
     uint32_t codes = 0;
+    float t[8], off = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int c = s > 0.0f ? __float2int_rn(__fdiv_rn(__fsub_rn(v[i], m), s)) : 0;
-        codes |= (uint32_t)max(0, min(15, c)) << (4 * i);
+    for (int i = 0; i < 8; i++) {
+        t[i] = fminf(fmaxf(__fmul_rn(__fsub_rn(v[i], m), r), 0.0f), 15.0f);
+        off = fmaxf(off, fabsf(__fsub_rn(t[i], __fsub_rn(__fadd_rn(t[i], big), big))));
     }
+    if (off > 0.4999f)
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = fminf(fmaxf(__fdiv_rn(__fsub_rn(v[i], m), s), 0.0f), 15.0f);
+#pragma unroll
+    for (int i = 0; i < 8; i++) codes |= (__float_as_uint(__fadd_rn(t[i], big)) & 15u) << (4 * i);
     return codes;
 }
 

@@ -2,15 +2,15 @@
  *
  * append: per head vector x of a row at position p, y = x * rsqrt(mean(x^2) + eps) * w; channel pairs (2 i, 2 i + 1) turned by the
  * angle p * base^(-2 i / 128); queries rounded to bf16, keys (turned) and values (as they come) quantised in groups of 32.
- * A warp holds a head vector, four channels a lane: the norm is one shuffle tree, the pairs are inside a lane, a group is eight
- * lanes.  All of it is in 32 bits up to the one rounding of the result; the angle is reduced in 64 (at position 32768 the
+ * Half a warp holds a head vector, eight channels a lane: the norm is one shuffle tree, the pairs are inside a lane, a group is four
+ * lanes.  (With a warp to a vector the issue slots were what bounded it: 193 instructions a vector.)  All of it is in 32 bits up to the one rounding of the result; the angle is reduced in 64 (at position 32768 the
  * fastest pair has turned 5215 times: 32 bits would leave it 2e-3 off). */
 #include <math.h>
 #include "kv4.cuh"
 
 namespace s2p {
 
-constexpr int KV4_ROW_WARPS = 8;
+constexpr int KV4_ROW_WARPS = 8, KV4_ROWS = 4, KV4_AHEAD = 3; /* warps and rows of a CTA; pairs of vectors whose loads a warp has under way */
 
 /* cosine and sine of pair i at position pos; per_pair = log2(base) / 64 */
 __device__ __forceinline__ float2 kv4_turn(int pos, int i, double per_pair) {
@@ -21,106 +21,168 @@ __device__ __forceinline__ float2 kv4_turn(int pos, int i, double per_pair) {
     return make_float2(c, s);
 }
 
-__global__ void __launch_bounds__(KV4_ROW_WARPS * 32)
-k_kv4_append(Kv4View cache, Kv4Rows b, const __nv_bfloat16* qkv, const __nv_bfloat16* q_norm, const __nv_bfloat16* k_norm, float eps,
+struct Kv4Place { int found, pos, page; }; /* of a row: whether an entry brings it, its position or -1, the page or -1 */
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4View& cache, const Kv4Rows& b, int row) {
+    Kv4Place p;
+    int seq = -1;
+    p.pos = -1;
+    p.found = row < b.rows && kv4_find(cache, b, row, seq, p.pos);
+    p.page = p.found && p.pos >= 0 ? kv4_page(cache, seq, p.pos) : -1;
+    return p;
+}
+
+/* A CTA has `rows` (up to KV4_ROWS) consecutive rows, whose places and angles it works out once, and its warps their pairs of head vectors in turn. */
+__global__ void __launch_bounds__(KV4_ROW_WARPS * 32, 4)
+k_kv4_append(Kv4View cache, Kv4Rows b, int rows, const __nv_bfloat16* qkv, const __nv_bfloat16* q_norm, const __nv_bfloat16* k_norm, float eps,
              double per_pair, __nv_bfloat16* q) {
-    __shared__ float2 turn[64];
-    __shared__ int sh[3];
-    const int row = blockIdx.x, lane = threadIdx.x & 31;
-    const int heads = cache.q_heads + 2 * cache.kv_heads, head = blockIdx.y * KV4_ROW_WARPS + (threadIdx.x >> 5);
+    __shared__ __align__(16) float2 turn[KV4_ROWS][64];
+    __shared__ Kv4Place place[KV4_ROWS];
+    const int row0 = blockIdx.x * rows, l = threadIdx.x & 15, second = (threadIdx.x >> 4) & 1;
+    const unsigned half = 0xFFFFu << (16 * second);
+    const int heads = cache.q_heads + 2 * cache.kv_heads, step = KV4_ROW_WARPS * gridDim.y, first = blockIdx.y * KV4_ROW_WARPS + (threadIdx.x >> 5);
     grid_wait();
     grid_release();
-    if (threadIdx.x == 0) {
-        int seq = -1, pos = -1;
-        sh[0] = kv4_find(cache, b, row, seq, pos);
-        sh[1] = pos;
-        sh[2] = pos >= 0 ? kv4_page(cache, seq, pos) : -1;
-    }
+    if (threadIdx.x < rows) place[threadIdx.x] = kv4_place(cache, b, row0 + threadIdx.x);
     __syncthreads();
-    if (!sh[0]) return;
-    const int pos = sh[1], page = sh[2];
-    if (threadIdx.x < 64) turn[threadIdx.x] = kv4_turn(max(pos, 0), threadIdx.x, per_pair);
+    for (int i = threadIdx.x; i < 64 * rows; i += KV4_ROW_WARPS * 32) turn[i >> 6][i & 63] = kv4_turn(max(place[i >> 6].pos, 0), i & 63, per_pair);
     __syncthreads();
-    if (head >= heads) return;
-
-    const bool is_q = head < cache.q_heads, is_v = head >= cache.q_heads + cache.kv_heads;
-    if (pos < 0) {
-        if (is_q) reinterpret_cast<uint2*>(q + ((size_t)row * cache.q_heads + head) * 128)[lane] = make_uint2(0, 0);
-        return;
-    }
-    if (!is_q && page < 0) return;
-    const uint2 raw = reinterpret_cast<const uint2*>(qkv + ((size_t)row * heads + head) * 128)[lane];
-    float x[4] = {bf_lo(raw.x), bf_hi(raw.x), bf_lo(raw.y), bf_hi(raw.y)};
-    if (!is_v) {
-        const __nv_bfloat16* w = is_q ? q_norm : k_norm;
-        if (w) {
-            const float sum = warp_tree_sum(fmaf(x[0], x[0], fmaf(x[1], x[1], fmaf(x[2], x[2], x[3] * x[3]))));
-            const float r = 1.0f / sqrtf(sum * (1.0f / 128.0f) + eps);
-            const uint2 g = reinterpret_cast<const uint2*>(w)[lane];
-            x[0] = x[0] * r * bf_lo(g.x); x[1] = x[1] * r * bf_hi(g.x);
-            x[2] = x[2] * r * bf_lo(g.y); x[3] = x[3] * r * bf_hi(g.y);
-        }
+    for (int r = 0; r < rows; r++) {
+        const int pos = place[r].pos, page = place[r].page;
+        if (!place[r].found) continue;
+        const uint4* from = reinterpret_cast<const uint4*>(qkv + (size_t)(row0 + r) * heads * 128) + l;
+        for (int i0 = first; 2 * i0 < heads; i0 += KV4_AHEAD * step) {
+            uint4 raws[KV4_AHEAD];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float2 t = turn[2 * lane + i];
-            const float a = x[2 * i], c = x[2 * i + 1];
-            x[2 * i] = a * t.x - c * t.y;
-            x[2 * i + 1] = c * t.x + a * t.y;
+            for (int k = 0; k < KV4_AHEAD; k++) {
+                const int head = 2 * (i0 + k * step) + second;
+                raws[k] = head < heads && pos >= 0 ? from[head * 16] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < KV4_AHEAD; k++) {
+                const int head = 2 * (i0 + k * step) + second;
+                const bool is_q = head < cache.q_heads, is_v = head >= cache.q_heads + cache.kv_heads;
+                if (head >= heads || (!is_q && page < 0)) continue;
+                const uint4 raw = raws[k];
+                float x[8] = {bf_lo(raw.x), bf_hi(raw.x), bf_lo(raw.y), bf_hi(raw.y), bf_lo(raw.z), bf_hi(raw.z), bf_lo(raw.w), bf_hi(raw.w)};
+                if (!is_v) {
+                    const __nv_bfloat16* w = is_q ? q_norm : k_norm;
+                    if (w) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+                        for (int off = 1; off < 16; off <<= 1) sum += __shfl_xor_sync(half, sum, off);
+                        const float n = rsqrtf(sum * (1.0f / 128.0f) + eps);
+                        const uint2 g0 = reinterpret_cast<const uint2*>(w)[2 * l], g1 = reinterpret_cast<const uint2*>(w)[2 * l + 1];
+                        const float g[8] = {bf_lo(g0.x), bf_hi(g0.x), bf_lo(g0.y), bf_hi(g0.y), bf_lo(g1.x), bf_hi(g1.x), bf_lo(g1.y), bf_hi(g1.y)};
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] *= n * g[i];
+                    }
+                    const float4 t0 = reinterpret_cast<const float4*>(turn[r])[2 * l], t1 = reinterpret_cast<const float4*>(turn[r])[2 * l + 1];
+                    const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        const float a = x[2 * h], d = x[2 * h + 1];
+                        x[2 * h] = a * c[h] - d * s[h];
+                        x[2 * h + 1] = d * c[h] + a * s[h];
+                    }
+                }
+                if (is_q) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        const __nv_bfloat162 z = __floats2bfloat162_rn(x[2 * h], x[2 * h + 1]);
+                        y[h] = *reinterpret_cast<const uint32_t*>(&z);
+                    }
+                    reinterpret_cast<uint4*>(q + ((size_t)(row0 + r) * cache.q_heads + head) * 128)[l] = make_uint4(y[0], y[1], y[2], y[3]);
+                    continue;
+                }
+                __half s, m;
+                const uint32_t codes = kv4_quantise(x, half, s, m);
+                const int in = pos % 16, j = l >> 2;
+                unsigned char* block = kv4_block(cache, page, head - cache.q_heads - (is_v ? cache.kv_heads : 0), pos);
+                if (is_v) {
+                    unsigned char* at = block + kv4_value_at(in, l);
+                    *reinterpret_cast<uint16_t*>(at) = (uint16_t)codes;
+                    *reinterpret_cast<uint16_t*>(at + 64) = (uint16_t)(codes >> 16);
+                } else *reinterpret_cast<uint32_t*>(block + kv4_key_at(in, l)) = codes;
+                if ((l & 3) == 0) {
+                    unsigned char* at = block + (is_v ? kv4_value_param_at(in, j) : kv4_key_param_at(in, j));
+                    *reinterpret_cast<__half*>(at) = s;
+                    *reinterpret_cast<__half*>(at + (is_v ? 128 : 8)) = m;
+                }
+            }
         }
     }
-    if (is_q) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-        reinterpret_cast<uint2*>(q + ((size_t)row * cache.q_heads + head) * 128)[lane] =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        return;
-    }
-    __half s, m;
-    const uint32_t codes = kv4_quantise(x, s, m);
-    const int i = pos % 16, j = lane >> 3;
-    unsigned char* block = kv4_block(cache, page, head - cache.q_heads - (is_v ? cache.kv_heads : 0), pos);
-    *reinterpret_cast<uint16_t*>(block + (is_v ? kv4_value_at(i, lane) : kv4_key_at(i, lane))) = (uint16_t)codes;
-    if ((lane & 7) == 0) {
-        unsigned char* at = block + (is_v ? kv4_value_param_at(i, j) : kv4_key_param_at(i, j));
-        *reinterpret_cast<__half*>(at) = s;
-        *reinterpret_cast<__half*>(at + (is_v ? 128 : 8)) = m;
-    }
+}
+
+/* Rows to a CTA and CTAs to them: several rows where there are many, several CTAs where there are few. */
+struct Kv4RowGrid { dim3 grid; int rows; };
+static Kv4RowGrid kv4_row_grid(int rows, int vectors) {
+    Kv4RowGrid g;
+    g.rows = rows >= 148 * KV4_ROWS ? KV4_ROWS : 1;
+    const int x = (rows + g.rows - 1) / g.rows, most = ((vectors + 1) / 2 + KV4_ROW_WARPS - 1) / KV4_ROW_WARPS;
+    const int want = (2 * 148 + x - 1) / x;
+    g.grid = dim3((unsigned)x, (unsigned)(want < most ? want : most));
+    return g;
 }
 
 extern "C" cudaError_t kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* qkv, const void* q_norm,
                                   const void* k_norm, float eps, float rope_base, void* q, cudaStream_t st) {
-    const int heads = c->q_heads + 2 * c->kv_heads;
-    return launch_after(k_kv4_append, dim3((unsigned)b->rows, (unsigned)((heads + KV4_ROW_WARPS - 1) / KV4_ROW_WARPS)), KV4_ROW_WARPS * 32, 0, st,
-                        kv4_view(*c, layer), kv4_rows(*b), static_cast<const __nv_bfloat16*>(qkv), static_cast<const __nv_bfloat16*>(q_norm),
-                        static_cast<const __nv_bfloat16*>(k_norm), eps, log2((double)rope_base) / 64.0, static_cast<__nv_bfloat16*>(q));
+    const Kv4RowGrid g = kv4_row_grid(b->rows, c->q_heads + 2 * c->kv_heads);
+    return launch_after(k_kv4_append, g.grid, KV4_ROW_WARPS * 32, 0, st, kv4_view(*c, layer), kv4_rows(*b), g.rows, static_cast<const __nv_bfloat16*>(qkv),
+                        static_cast<const __nv_bfloat16*>(q_norm), static_cast<const __nv_bfloat16*>(k_norm), eps > 1e-37f ? eps : 1e-37f /* a row of zeros stays one */, log2((double)rope_base) / 64.0,
+                        static_cast<__nv_bfloat16*>(q));
 }
 
-/* One warp per (row, kv head, keys or values): the inverse of append's stores. */
-__global__ void __launch_bounds__(KV4_ROW_WARPS * 32) k_kv4_read(Kv4View cache, Kv4Rows b, __nv_bfloat16* k, __nv_bfloat16* v) {
-    const int row = blockIdx.x, lane = threadIdx.x & 31, unit = blockIdx.y * KV4_ROW_WARPS + (threadIdx.x >> 5);
-    if (unit >= 2 * cache.kv_heads) return;
+/* The inverse of append's stores, its rows and head vectors cut the same way; a pair is a kv head's key and value. */
+__global__ void __launch_bounds__(KV4_ROW_WARPS * 32) k_kv4_read(Kv4View cache, Kv4Rows b, int rows, __nv_bfloat16* k_out, __nv_bfloat16* v_out) {
+    __shared__ Kv4Place place[KV4_ROWS];
+    const int row0 = blockIdx.x * rows, l = threadIdx.x & 15, is_v = (threadIdx.x >> 4) & 1;
+    const int step = KV4_ROW_WARPS * gridDim.y, first = blockIdx.y * KV4_ROW_WARPS + (threadIdx.x >> 5);
     grid_wait();
     grid_release();
-    int seq = -1, pos = -1;
-    if (!kv4_find(cache, b, row, seq, pos)) return;
-    const int head = unit >> 1, is_v = unit & 1, page = pos >= 0 ? kv4_page(cache, seq, pos) : -1;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (page >= 0) {
-        const int i = pos % 16, j = lane >> 3;
-        const unsigned char* block = kv4_block(cache, page, head, pos);
-        const uint32_t codes = *reinterpret_cast<const uint16_t*>(block + (is_v ? kv4_value_at(i, lane) : kv4_key_at(i, lane)));
-        const unsigned char* at = block + (is_v ? kv4_value_param_at(i, j) : kv4_key_param_at(i, j));
-        const float s = __half2float(*reinterpret_cast<const __half*>(at)), m = __half2float(*reinterpret_cast<const __half*>(at + (is_v ? 128 : 8)));
+    if (threadIdx.x < rows) place[threadIdx.x] = kv4_place(cache, b, row0 + threadIdx.x);
+    __syncthreads();
+    constexpr int AHEAD = 4; /* heads whose loads a warp has under way */
+    for (int i0 = first; i0 < rows * cache.kv_heads; i0 += AHEAD * step) {
+        uint32_t codes[AHEAD];
+        __half s[AHEAD], m[AHEAD];
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = fmaf(s, (float)((codes >> (4 * e)) & 15u), m);
+        for (int k = 0; k < AHEAD; k++) {
+            const int i = i0 + k * step, r = min(i / cache.kv_heads, rows - 1), head = i - r * cache.kv_heads, pos = place[r].pos, page = place[r].page;
+            codes[k] = 0;
+            s[k] = m[k] = __half(0.0f);
+            if (i < rows * cache.kv_heads && page >= 0) {
+                const int in = pos % 16, j = l >> 2;
+                const unsigned char* block = kv4_block(cache, page, head, pos);
+                const unsigned char* at = block + (is_v ? kv4_value_param_at(in, j) : kv4_key_param_at(in, j));
+                s[k] = *reinterpret_cast<const __half*>(at);
+                m[k] = *reinterpret_cast<const __half*>(at + (is_v ? 128 : 8));
+                if (is_v) codes[k] = *reinterpret_cast<const uint16_t*>(block + kv4_value_at(in, l)) | (uint32_t)*reinterpret_cast<const uint16_t*>(block + kv4_value_at(in, l) + 64) << 16;
+                else codes[k] = *reinterpret_cast<const uint32_t*>(block + kv4_key_at(in, l));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const int i = i0 + k * step, r = min(i / cache.kv_heads, rows - 1), head = i - r * cache.kv_heads;
+            if (i >= rows * cache.kv_heads || !place[r].found) continue;
+            const float sf = __half2float(s[k]), mf = __half2float(m[k]);
+            uint32_t y[4];
+#pragma unroll
+            for (int h = 0; h < 4; h++) {
+                const __nv_bfloat162 z = __floats2bfloat162_rn(fmaf(sf, (float)((codes[k] >> (8 * h)) & 15u), mf), fmaf(sf, (float)((codes[k] >> (8 * h + 4)) & 15u), mf));
+                y[h] = *reinterpret_cast<const uint32_t*>(&z);
+            }
+            reinterpret_cast<uint4*>((is_v ? v_out : k_out) + ((size_t)(row0 + r) * cache.kv_heads + head) * 128)[l] = make_uint4(y[0], y[1], y[2], y[3]);
+        }
     }
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-    reinterpret_cast<uint2*>((is_v ? v : k) + ((size_t)row * cache.kv_heads + head) * 128)[lane] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
 extern "C" cudaError_t kv4_read(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, void* k, void* v, cudaStream_t st) {
-    return launch_after(k_kv4_read, dim3((unsigned)b->rows, (unsigned)((2 * c->kv_heads + KV4_ROW_WARPS - 1) / KV4_ROW_WARPS)), KV4_ROW_WARPS * 32, 0,
-                        st, kv4_view(*c, layer), kv4_rows(*b), static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+    const Kv4RowGrid g = kv4_row_grid(b->rows, 2 * c->kv_heads);
+    return launch_after(k_kv4_read, g.grid, KV4_ROW_WARPS * 32, 0, st, kv4_view(*c, layer), kv4_rows(*b), g.rows, static_cast<__nv_bfloat16*>(k),
+                        static_cast<__nv_bfloat16*>(v));
 }
 
 }  // namespace s2p
