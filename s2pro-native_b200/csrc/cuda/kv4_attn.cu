@@ -363,17 +363,16 @@ __device__ __forceinline__ void ka_store(__nv_bfloat16* to, float4 v, float sum)
 
 template <int NT>
 __global__ void __launch_bounds__(KA_THREADS, 1)
-k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloat16* out, KaParts parts) {
+k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __nv_bfloat16* q, __nv_bfloat16* out, KaParts parts) {
     constexpr int COLS = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sh_max[KA_WARPS][COLS], sh_sum[KA_WARPS][COLS];
-    __shared__ unsigned sh_scan[KA_WARPS];
+    __shared__ struct { unsigned by_warp, workers, longest, share, more; } sh_line;
     __shared__ int sh_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem + warp * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
     float* merge = reinterpret_cast<float*>(smem + KA_RING_BYTES);
     const KaBatch batch = ka_batch(smem + KA_RING_BYTES + KA_MERGE_BYTES, b.n);
-    const int group = cache.q_heads / cache.kv_heads, rows_per = max(1, COLS / group);
     const int capacity = cache.stride * S2P_B200_KV4_PAGE;
 
     grid_wait();
@@ -387,92 +386,82 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloa
     };
     auto units_of = [&](int e) { /* entries of more rows than `few` are another kernel's */
         const int rows = batch.start[e + 1] - batch.start[e];
-        return rows > few ? 0 : (rows + rows_per - 1) / rows_per * cache.kv_heads;
+        return rows > few || !rows ? 0 : rows <= rows_per ? cache.kv_heads : (rows + rows_per - 1) / rows_per * cache.kv_heads;
     };
-    const int per = b.n / KA_THREADS + 1; /* entries of a thread, the end of the last among them */
-    {
-        int top = 0;
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
-            const int r = b.row0[e];
-            if (e < b.n) {
-                const int seq = b.seqs[e], p0 = b.pos0[e];
-                batch.seq[e] = seq;
-                batch.first[e] = (unsigned)seq < (unsigned)cache.max_seqs && p0 <= (1 << 30) ? p0 : -1;
-            }
-            top = max(top, min(r, b.rows));
-            batch.start[e] = min(r, b.rows);
+    /* Brought by all, worked out by one warp, 32 entries at a time: two barriers.  (By all warps, with a barrier for every sum, 0.6 us more.) */
+    for (int e = tid; e <= b.n; e += KA_THREADS) {
+        const int r = b.row0[e];
+        if (e < b.n) {
+            const int seq = b.seqs[e], p0 = b.pos0[e];
+            batch.seq[e] = seq;
+            batch.first[e] = (unsigned)seq < (unsigned)cache.max_seqs && p0 <= (1 << 30) ? p0 : -1;
         }
-        int before = top;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(S2P_FULL_MASK, before, off);
-            if (lane >= off) before = max(before, o);
-        }
-        if (lane == 31) sh_scan[warp] = (unsigned)before;
-        before = __shfl_up_sync(S2P_FULL_MASK, before, 1);
-        if (lane == 0) before = 0;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) before = max(before, w < warp ? (int)sh_scan[w] : 0);
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) batch.start[e] = before = max(before, batch.start[e]);
-        __syncthreads();
+        batch.start[e] = min(r, b.rows);
     }
-    /* before[e] and the sum over all entries of what `of` gives for each */
-    auto line_up = [&](auto of) {
-        unsigned sum = 0, all = 0;
-        for (int i = 0, e = tid * per; i < per && e < b.n; i++, e++) sum += of(e);
-        unsigned at = sum;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
-            if (lane >= off) at += o;
-        }
-        __syncthreads(); /* upto and sh_scan may be read still */
-        if (lane == 31) sh_scan[warp] = at;
-        at -= sum;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) {
-            at += w < warp ? sh_scan[w] : 0;
-            all += sh_scan[w];
-        }
-        for (int i = 0, e = tid * per; i < per && e <= b.n; i++, e++) {
-            batch.upto[e] = at;
-            if (e < b.n) at += of(e);
-        }
-        __syncthreads();
-        return all;
-    };
-    const unsigned total = line_up([&](int e) { return (unsigned)units_of(e) * (unsigned)blocks_of(e); });
-    unsigned units = 0;
-    for (int i = 0, e = tid * per; i < per && e < b.n; i++, e++) units += (unsigned)units_of(e);
-    units = (unsigned)__reduce_add_sync(S2P_FULL_MASK, units);
-    if (lane == 0) sh_scan[warp] = units;
     __syncthreads();
-    units = 0;
+    if (warp == 0) {
+        auto before = [&](unsigned v, unsigned& carry) { /* carry + the lanes before this one; carry goes on */
+            unsigned at = v;
 #pragma unroll
-    for (int w = 0; w < KA_WARPS; w++) units += sh_scan[w];
-    if (!total) return;
-
-    /* Few units on short sequences: each is cut into parts, a CTA to a part, its warps a stretch of it each.  Otherwise warps work by
-     * themselves (no barriers, but a partial for every warp) on equal stretches of the line of all units' blocks. */
-    const bool by_warp = total >= gridDim.x * KA_WARPS * KA_LONG || 2 * units > gridDim.x;
-    unsigned begin, end, share = 1, more = 0, longest = 1;
-    if (by_warp) {
-        const unsigned workers = min(gridDim.x * KA_WARPS, (total + KA_LEAST_WARP - 1) / KA_LEAST_WARP), worker = warp * gridDim.x + blockIdx.x;
-        if (worker >= workers) return;
-        /* worker w has `share` blocks of the line, the first `more` workers one more */
-        share = total / workers;
-        more = total - share * workers;
-        begin = share * worker + min(worker, more);
-        end = begin + share + (worker < more);
-    } else {
-        longest = max((unsigned)KA_LEAST_CTA, (total + gridDim.x - units - 1) / (gridDim.x - units)); /* so there are at most gridDim.x parts */
-        const unsigned parts_all = line_up([&](int e) { return (unsigned)units_of(e) * ((blocks_of(e) + longest - 1) / longest); });
-        begin = blockIdx.x;
-        end = begin + 1;
-        if (begin >= parts_all) return;
+            for (int off = 1; off < 32; off <<= 1) {
+                const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
+                if (lane >= off) at += o;
+            }
+            const unsigned mine = carry + at - v;
+            carry += __shfl_sync(S2P_FULL_MASK, at, 31);
+            return mine;
+        };
+        int top = 0;
+        for (int e0 = 0; e0 <= b.n; e0 += 32) {
+            const int e = e0 + lane;
+            int r = max(e <= b.n ? batch.start[e] : 0, top);
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(S2P_FULL_MASK, r, off);
+                if (lane >= off) r = max(r, o);
+            }
+            if (e <= b.n) batch.start[e] = r;
+            top = __shfl_sync(S2P_FULL_MASK, r, 31);
+        }
+        __syncwarp();
+        unsigned total = 0, units = 0;
+        for (int e0 = 0; e0 <= b.n; e0 += 32) {
+            const int e = e0 + lane;
+            const unsigned u = e < b.n ? (unsigned)units_of(e) : 0u;
+            units += __reduce_add_sync(S2P_FULL_MASK, u);
+            const unsigned at = before(u ? u * (unsigned)blocks_of(e) : 0u, total);
+            if (e <= b.n) batch.upto[e] = at;
+        }
+        /* Few units on short sequences: each is cut into parts, a CTA to a part, its warps a stretch of it each.  Otherwise warps work by
+         * themselves (no barriers, but a partial for every warp) on equal stretches of the line of all units' blocks. */
+        const bool by_warp = total >= gridDim.x * KA_WARPS * KA_LONG || 2 * units > gridDim.x;
+        unsigned workers = min(gridDim.x * KA_WARPS, (total + KA_LEAST_WARP - 1) / KA_LEAST_WARP), longest = 1;
+        if (!by_warp) {
+            longest = max((unsigned)KA_LEAST_CTA, (total + gridDim.x - units - 1) / (gridDim.x - units)); /* so there are at most gridDim.x parts */
+            workers = 0;
+            __syncwarp();
+            for (int e0 = 0; e0 <= b.n; e0 += 32) {
+                const int e = e0 + lane;
+                const unsigned u = e < b.n ? (unsigned)units_of(e) : 0u;
+                const unsigned at = before(u ? u * ((blocks_of(e) + longest - 1) / longest) : 0u, workers);
+                if (e <= b.n) batch.upto[e] = at;
+            }
+        }
+        if (lane == 0) {
+            sh_line.by_warp = by_warp;
+            sh_line.workers = workers;
+            sh_line.longest = longest;
+            /* worker w of the line has `share` blocks, the first `more` workers one more */
+            sh_line.share = by_warp && workers ? total / workers : 1;
+            sh_line.more = by_warp ? total - sh_line.share * workers : 0;
+        }
     }
+    __syncthreads();
+    const bool by_warp = sh_line.by_warp;
+    const unsigned workers = sh_line.workers, longest = sh_line.longest, share = sh_line.share, more = sh_line.more;
+    const unsigned worker = by_warp ? warp * gridDim.x + blockIdx.x : blockIdx.x;
+    if (worker >= workers) return;
+    const unsigned begin = by_warp ? share * worker + min(worker, more) : worker, end = by_warp ? begin + share + (worker < more) : begin + 1;
     auto worker_of = [&](unsigned x) { return x < (share + 1) * more ? x / (share + 1) : more + (x - (share + 1) * more) / share; };
 
     int e = 0;
@@ -484,72 +473,90 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloa
         }
         e = lo;
     }
-    for (unsigned cur = begin; cur < end;) {
+    struct Segment { /* the stretch's part in one unit */
+        int row, n_rows, r0, head, seq, p0, seen, least, blocks, x0, x1, w0, w1; /* blocks x0 .. x1 - 1 of `blocks`; the workers of the unit */
+        int xa, xb, pieces;                                                    /* this warp's blocks, in pieces that end where a page does */
+    };
+    auto segment = [&](unsigned cur) {
+        Segment s;
         while (batch.upto[e + 1] <= cur) e++; /* entries without rows */
-        const int blocks = blocks_of(e), rows = batch.start[e + 1] - batch.start[e];
+        const int rows = batch.start[e + 1] - batch.start[e];
+        s.blocks = blocks_of(e);
         const unsigned inside = cur - batch.upto[e];
         unsigned unit;
-        int x0, x1, w0, w1; /* the blocks of this stretch, and the workers of the unit */
         if (by_warp) {
-            unit = inside / (unsigned)blocks;
-            x0 = (int)(inside - unit * (unsigned)blocks);
-            x1 = x0 + (int)min((unsigned)(blocks - x0), end - cur);
-            w0 = (int)worker_of(cur - (unsigned)x0);
-            w1 = (int)worker_of(cur - (unsigned)x0 + (unsigned)blocks - 1);
+            unit = inside / (unsigned)s.blocks;
+            s.x0 = (int)(inside - unit * (unsigned)s.blocks);
+            s.x1 = s.x0 + (int)min((unsigned)(s.blocks - s.x0), end - cur);
+            s.w0 = (int)worker_of(cur - (unsigned)s.x0);
+            s.w1 = (int)worker_of(cur - (unsigned)s.x0 + (unsigned)s.blocks - 1);
+            s.xa = s.x0;
+            s.xb = s.x1;
         } else {
-            const int cuts = (int)((blocks + longest - 1) / longest);
+            const int cuts = (int)((s.blocks + longest - 1) / longest);
             unit = inside / (unsigned)cuts;
-            const int cut = (int)(inside - unit * (unsigned)cuts), piece = blocks / cuts, rest = blocks - piece * cuts;
-            x0 = piece * cut + min(cut, rest);
-            x1 = x0 + piece + (cut < rest);
-            w0 = (int)cur - cut;
-            w1 = w0 + cuts - 1;
+            const int cut = (int)(inside - unit * (unsigned)cuts), piece = s.blocks / cuts, rest = s.blocks - piece * cuts;
+            s.x0 = piece * cut + min(cut, rest);
+            s.x1 = s.x0 + piece + (cut < rest);
+            s.w0 = (int)cur - cut;
+            s.w1 = s.w0 + cuts - 1;
+            const int each = (s.x1 - s.x0) / KA_WARPS, over = (s.x1 - s.x0) % KA_WARPS;
+            s.xa = s.x0 + each * warp + min(warp, over);
+            s.xb = s.xa + each + (warp < over);
         }
-        const int chunk = (int)(unit / (unsigned)cache.kv_heads), head = (int)unit - chunk * cache.kv_heads;
-        const int r0 = chunk * rows_per, n_rows = min(rows_per, rows - r0), columns = n_rows * group;
-        const int row = batch.start[e] + r0, seq = batch.seq[e], p0 = batch.first[e];
-        const int seen = seen_by(p0, r0 + n_rows - 1), least = seen_by(p0, r0); /* by the last row and the first */
-        const size_t q_stride = (size_t)cache.q_heads * 128;
-
-        /* This warp's blocks, in pieces that end where a page does; lane i keeps the page of the (32 n + i)-th piece. */
-        const int xa = by_warp ? x0 : x0 + (x1 - x0) / KA_WARPS * warp + min(warp, (x1 - x0) % KA_WARPS), xb = by_warp ? x1 : xa + (x1 - x0) / KA_WARPS + (warp < (x1 - x0) % KA_WARPS);
-        const int pieces = xb > xa ? (xb - 1) / KA_PIECE - xa / KA_PIECE + 1 : 0;
-        int page_of = -1;
-        unsigned absent = 0; /* stages without a page */
-        auto fetch = [&](int i) {
-            if (i < pieces) {
-                const int at = xa / KA_PIECE + i;
-                if ((i & 31) == 0) page_of = i + lane < pieces ? kv4_page(cache, seq, (at + lane) * KA_PIECE * 16) : -1;
-                const int page = __shfl_sync(S2P_FULL_MASK, page_of, i & 31);
-                const int from = max(xa, KA_PIECE * at), n = min(min(xb, KA_PIECE * (at + 1)), (seen + 15) / 16) - from; /* (an entry that sees nothing has a block, too) */
-                const unsigned bit = 1u << (i % KA_STAGES);
-                if (page >= 0 && n > 0) {
-                    const unsigned char* src = kv4_block(cache, page, head, from * 16) + lane * 16;
-                    uint32_t dst = smem_u32(ring) + (i % KA_STAGES) * KA_PIECE * KV4_BLOCK_BYTES + lane * 16;
-                    for (int x = 0; x < n; x++, src += KV4_BLOCK_BYTES, dst += KV4_BLOCK_BYTES)
+        s.pieces = s.xb > s.xa ? (s.xb - 1) / KA_PIECE - s.xa / KA_PIECE + 1 : 0;
+        const int chunk = (int)(unit / (unsigned)cache.kv_heads);
+        s.head = (int)unit - chunk * cache.kv_heads;
+        s.r0 = chunk * rows_per;
+        s.n_rows = min(rows_per, rows - s.r0);
+        s.row = batch.start[e] + s.r0;
+        s.seq = batch.seq[e];
+        s.p0 = batch.first[e];
+        s.seen = seen_by(s.p0, s.r0 + s.n_rows - 1); /* by the last row */
+        s.least = seen_by(s.p0, s.r0);               /* ... and the first */
+        return s;
+    };
+    int page_of = -1;    /* lane i keeps the page of the (32 n + i)-th piece */
+    unsigned absent = 0; /* stages without a page */
+    auto fetch = [&](const Segment& s, int i) {
+        if (i < s.pieces) {
+            const int at = s.xa / KA_PIECE + i;
+            if ((i & 31) == 0) page_of = i + lane < s.pieces ? kv4_page(cache, s.seq, (at + lane) * KA_PIECE * 16) : -1;
+            const int page = __shfl_sync(S2P_FULL_MASK, page_of, i & 31);
+            const int from = max(s.xa, KA_PIECE * at), n = min(min(s.xb, KA_PIECE * (at + 1)), (s.seen + 15) / 16) - from; /* (an entry that sees nothing has a block, too) */
+            const unsigned bit = 1u << (i % KA_STAGES);
+            if (page >= 0 && n > 0) {
+                const unsigned char* src = kv4_block(cache, page, s.head, from * 16) + lane * 16;
+                uint32_t dst = smem_u32(ring) + (i % KA_STAGES) * KA_PIECE * KV4_BLOCK_BYTES + lane * 16;
+                for (int x = 0; x < n; x++, src += KV4_BLOCK_BYTES, dst += KV4_BLOCK_BYTES)
 #pragma unroll
-                        for (int k = 0; k < KV4_BLOCK_BYTES / 512; k++)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 512), "l"(src + k * 512) : "memory");
-                    absent &= ~bit;
-                } else absent |= bit;
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (int i = 0; i < KA_STAGES - 1; i++) fetch(i);
+                    for (int k = 0; k < KV4_BLOCK_BYTES / 512; k++)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 512), "l"(src + k * 512) : "memory");
+                absent &= ~bit;
+            } else absent |= bit;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 
+    const size_t q_stride = (size_t)cache.q_heads * 128;
+    unsigned cur = begin;
+    Segment s = segment(cur);
+#pragma unroll
+    for (int i = 0; i < KA_STAGES - 1; i++) fetch(s, i);
+    for (;;) {
+        const int columns = s.n_rows * group, row = s.row, head = s.head, r0 = s.r0, p0 = s.p0, seen = s.seen;
         KaQuery<NT> query;
         ka_load_query<NT>(query, q + (size_t)row * q_stride + (size_t)head * group * 128, q_stride, group, columns, lane);
         KaState<NT> z;
         ka_clear(z);
-        for (int i = 0; i < pieces; i++) {
-            fetch(i + KA_STAGES - 1);
+        for (int i = 0; i < s.pieces; i++) {
+            fetch(s, i + KA_STAGES - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(KA_STAGES - 1) : "memory");
             __syncwarp();
             if (!(absent >> (i % KA_STAGES) & 1)) {
                 unsigned char* blk = ring + (i % KA_STAGES) * KA_PIECE * KV4_BLOCK_BYTES;
-                int x = max(xa, KA_PIECE * (xa / KA_PIECE + i));
-                const int to = min(min(xb, KA_PIECE * (xa / KA_PIECE + i + 1)), (seen + 15) / 16), plain = min(to, least / 16); /* blocks that every row sees whole */
+                int x = max(s.xa, KA_PIECE * (s.xa / KA_PIECE + i));
+                const int to = min(min(s.xb, KA_PIECE * (s.xa / KA_PIECE + i + 1)), (seen + 15) / 16), plain = min(to, s.least / 16); /* blocks that every row sees whole */
                 for (; x < to; x += 2, blk += 2 * KV4_BLOCK_BYTES) {
                     const int first = x * 16;
                     if (first + 32 > seen) { /* nobody has written what lies behind the last position: it must not meet a zero weight as NaN */
@@ -571,7 +578,16 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloa
             }
             __syncwarp();
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        /* the stretch's next unit is on its way while this one's result is written and, where it is shared, put together */
+        const Segment done = s;
+        const unsigned slot_at = cur;
+        cur += by_warp ? s.x1 - s.x0 : 1;
+        const bool go_on = cur < end;
+        if (go_on) {
+            s = segment(cur);
+#pragma unroll
+            for (int i = 0; i < KA_STAGES - 1; i++) fetch(s, i);
+        }
 
         /* the m term of a group to the lanes that hold its channels */
         float m_term[NT][2][4];
@@ -587,8 +603,9 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloa
             return make_float4(fmaf(z.o[nt][2 * j][c], 16777216.0f, m), fmaf(z.o[nt][2 * j][c + 2], 1048576.0f, m), fmaf(z.o[nt][2 * j + 1][c], 16777216.0f, m),
                                fmaf(z.o[nt][2 * j + 1][c + 2], 1048576.0f, m));
         };
-        const bool whole = x0 == 0 && x1 == blocks;
-        const size_t slot = by_warp ? 2 * (size_t)(warp * gridDim.x + blockIdx.x) + (x0 == 0 ? 1 : 0) : (size_t)cur;
+        const bool whole = done.x0 == 0 && done.x1 == done.blocks;
+        const int w0 = done.w0, w1 = done.w1;
+        const size_t slot = by_warp ? 2 * (size_t)(warp * gridDim.x + blockIdx.x) + (done.x0 == 0 ? 1 : 0) : (size_t)slot_at;
         unsigned* arrived = parts.arrived + (size_t)row * cache.kv_heads + head;
         auto out_of = [&](int col) { return out + (size_t)(row + col / group) * q_stride + (size_t)(head * group + col % group) * 128; };
 
@@ -703,7 +720,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloa
                 __syncthreads();
             }
         }
-        cur += by_warp ? x1 - x0 : 1;
+        if (!go_on) break;
     }
 }
 
@@ -729,9 +746,9 @@ static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
     p.o = reinterpret_cast<float*>(area);
     p.max = p.o + (size_t)KV4_PARTS * 128;
     p.sum = p.max + KV4_PARTS;
-    const int grid = sms[dev], most = KV4_PARTS / (2 * KA_WARPS * 8 * NT);
+    const int group = c->q_heads / c->kv_heads, grid = sms[dev], most = KV4_PARTS / (2 * KA_WARPS * 8 * NT);
     return launch_after(k_kv4_attn<NT>, dim3((unsigned)(grid < most ? grid : most)), KA_THREADS, smem, st, kv4_view(*c, layer), kv4_rows(*b), few,
-                        static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), p);
+                        group, 8 * NT > group ? 8 * NT / group : 1, static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), p);
 }
 
 extern "C" cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* q, void* out, cudaStream_t st) {
@@ -742,7 +759,8 @@ extern "C" cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_b
         const cudaError_t e = kv4_slices(c, b, layer, few, q, out, st);
         if (e != cudaSuccess || !few) return e;
     }
-    return (few < most ? few : most) * group <= 8 ? launch_attn<1>(c, b, layer, few, q, out, st) : launch_attn<2>(c, b, layer, few, q, out, st);
+    /* next to slices most entries bring a single token, and those of a few rows read their sequence a few times */
+    return few < most || most * group <= 8 ? launch_attn<1>(c, b, layer, few, q, out, st) : launch_attn<2>(c, b, layer, few, q, out, st);
 }
 
 }  // namespace s2p
