@@ -32,7 +32,10 @@ constexpr int KA_RING_BYTES = KA_WARPS * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
 constexpr int KA_PASS = 4;                                         /* columns merged at a time */
 constexpr int KA_MERGE_BYTES = KA_WARPS * KA_PASS * 128 * 4;
 constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 4;           /* blocks that make a worker worth its while */
-constexpr int KA_FEW = 32;                                         /* (row, head) columns of a kv head that are still single tokens' work */
+/* (Row, head) columns of a kv head up to which an entry is this kernel's rather than that of the tensor cores: alone, and next to longer slices, where
+ * most bring a token.  us here and there, 32 / 8 heads: 4, 16, 32, 64 rows of one sequence at 1100 positions 16.9, 18.2, 19.5, 42 and 16.4, 18.1,
+ * 20.3, 24.6; at 8000 positions 19.9, 27.6, 52, 61 and 27.9, 29.3, 33.4, 41.8; 4, 8, 16 rows of 16 sequences at 4000 53, 57, 82 and 72, 73, 75. */
+constexpr int KA_FEW = 64, KA_FEW_BESIDE = 32;
 constexpr int KA_LONG = 20;                                        /* blocks of a warp from which on warps work by themselves */
 
 struct KaBatch { /* in shared memory, [n (+ 1)] */
@@ -755,7 +758,7 @@ extern "C" cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_b
     const int group = c->q_heads / c->kv_heads, most = b->max_rows < b->rows ? b->max_rows : b->rows;
     int few = INT_MAX;
     if (most * group > KA_FEW && kv4_slices_serve(c, b)) {
-        few = b->n == 1 ? 0 : KA_FEW / group; /* the rows of an entry are known on the device alone: a batch of several may need both kernels */
+        few = b->n == 1 ? 0 : KA_FEW_BESIDE / group; /* the rows of an entry are known on the device alone: a batch of several may need both kernels */
         const cudaError_t e = kv4_slices(c, b, layer, few, q, out, st);
         if (e != cudaSuccess || !few) return e;
     }
