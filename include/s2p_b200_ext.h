@@ -132,10 +132,10 @@ typedef struct {
     int32_t* table;   /* [max_seqs][table_stride]: page of positions 64 j .. 64 j + 63; an entry outside the pool (-1) holds nothing */
     int32_t* lens;    /* [max_seqs] positions held; table entries behind them are -1 */
     int32_t* refs;    /* [n_pages] table entries that name the page; 0 = free */
-    void* work;       /* 256-byte aligned; zeroed once by the caller, before its first use */
+    void* work;       /* 256-byte aligned; zeroed once by the caller, before its first use; caches may share one */
     size_t work_bytes;
-    int n_pages, layers, kv_heads, q_heads; /* q_heads a multiple of kv_heads, at most 16 times as many; width 128 */
-    int max_seqs, table_stride;
+    int n_pages, layers, kv_heads, q_heads; /* up to 2^22 pages; q_heads a multiple of kv_heads, at most 16 times as many; width 128 */
+    int max_seqs, table_stride;             /* table_stride up to 2^24 */
 } s2p_b200_kv4;
 
 /* The rows of a tick or a prompt slice: entry b brings rows row0[b] .. row0[b + 1] - 1 of the activations, at positions
@@ -154,7 +154,8 @@ typedef struct {
 size_t s2p_b200_kv4_page_bytes(int layers, int kv_heads);
 /* workspace of every call on this cache, attention with batches of up to `rows` rows; 0 if the cache's sizes cannot be served */
 size_t s2p_b200_kv4_work_bytes(const s2p_b200_kv4* c, int rows);
-/* S2P_ERR_INTERNAL if a bounded wait of an earlier call on this workspace gave up (its rows are lost), once; waits for the stream */
+/* S2P_ERR_INTERNAL if a bounded wait of an attention call on this workspace gave up, once; rows of the calls since the status was last asked for may
+ * be lost.  Waits for the stream (so not under capture). */
 s2p_status s2p_b200_kv4_status(const s2p_b200_kv4* c, cudaStream_t stream);
 
 /* Room for the batch's rows: pos0 = positions held, lens += rows, and free pages (lowest first, in the batch's order) for
@@ -172,7 +173,9 @@ s2p_status s2p_b200_kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
                                const s2p_bf16* k_norm, float eps, float rope_base, s2p_bf16* q, cudaStream_t stream);
 
 /* out [rows, q_heads * 128]: softmax(q k / sqrt(128)) v over the positions of the row's sequence up to its own that have a
- * page; zeros where there is none.  rows * kv_heads * table_stride is at most 2^29. */
+ * page; zeros where there is none.  out may be q.  Queries are below 2^100 in magnitude; a NaN or an infinity in a head's query
+ * makes that head of the row NaN.  rows * kv_heads * table_stride is at most 2^29.  Slices take a kernel whose waits are
+ * bounded: see s2p_b200_kv4_status. */
 s2p_status s2p_b200_kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const s2p_bf16* q, s2p_bf16* out,
                                   cudaStream_t stream);
 

@@ -13,28 +13,21 @@
 #define KV4_MAX_LINE (1 << 29)   /* rows * kv_heads * table_stride of an attention call: its blocks are counted in 32 bits */
 
 /* The workspace: status word | one area for either the partials of a split attention or the lists of the page operators |
- * arrival counters of the split attention, zero between calls.  Only the last part's size goes by the rows, so that calls
- * with different numbers of rows agree on where everything is. */
+ * arrival counters of the split attention, zero between calls.  Everything is at the same place whatever the cache and the
+ * number of rows, so that calls on several caches can use one workspace in turn. */
 #define KV4_STATUS_BYTES 256
 #define KV4_PARTS (2 * 320 * 8 * 8) /* columns of partials: two for each of 8 columns of 8 warps of up to 320 CTAs; 128 + 2 floats each */
+#define KV4_SLICE_CTAS 160          /* CTAs of a slices' launch; two partials of 256 rows each, and a few words */
+#define KV4_SLICE_PART_FLOATS (256 * (128 + 2) + 8)
+#define KV4_AREA_BYTES ((size_t)2 * KV4_SLICE_CTAS * KV4_SLICE_PART_FLOATS * sizeof(float))
+#define KV4_MAX_PAGES (1 << 22) /* the page operators keep 8 bytes a page and a little more in the area: a pair of pages per move, a number per page */
 
 #ifdef __cplusplus
 namespace s2p {
 extern "C" {
 #endif
 
-#define KV4_SLICE_CTAS 160           /* CTAs of a slices' launch; two partials of 256 rows each */
-
-/* Bytes of the area.  The page operators keep a few words, a pair of pages per move and a new number per page. */
-static inline size_t kv4_area_bytes(int n_pages) {
-    const size_t tokens = (size_t)KV4_PARTS * (128 + 2) * sizeof(float), slices = (size_t)2 * KV4_SLICE_CTAS * (256 * (128 + 2) + 8) * sizeof(float);
-    const size_t part = tokens > slices ? tokens : slices;
-    const size_t lists = 256 + ((size_t)n_pages / 2 + 1 + S2P_B200_KV4_MAX_LIST) * 8 + (size_t)n_pages * 4;
-    return ((part > lists ? part : lists) + 255) / 256 * 256;
-}
-static inline size_t kv4_work_bytes(int n_pages, int rows, int kv_heads) {
-    return KV4_STATUS_BYTES + kv4_area_bytes(n_pages) + (size_t)rows * (size_t)kv_heads * sizeof(unsigned);
-}
+static inline size_t kv4_work_bytes(int rows, int kv_heads) { return KV4_STATUS_BYTES + KV4_AREA_BYTES + (size_t)rows * (size_t)kv_heads * sizeof(unsigned); }
 cudaError_t kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const void* qkv, const void* q_norm, const void* k_norm,
                        float eps, float rope_base, void* q, cudaStream_t st);
 cudaError_t kv4_read(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, void* k, void* v, cudaStream_t st);
@@ -42,6 +35,7 @@ cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, in
 /* slices of more than `few` rows, where the batch's chunks fit in shared memory */
 int kv4_slices_serve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b);
 cudaError_t kv4_slices(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, int few, const void* q, void* out, cudaStream_t st);
+cudaError_t kv4_slices_set_wait_ns(unsigned long long ns); /* test hook: deadline of that kernel's bounded waits */
 cudaError_t kv4_reserve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int32_t* info, cudaStream_t st);
 cudaError_t kv4_fork(const s2p_b200_kv4* c, const int32_t* parents, const int32_t* children, const int32_t* tokens, int n, int32_t* info,
                      cudaStream_t st);

@@ -307,6 +307,7 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
 }
 
 /* Partial results.  CTAs: slot w for part w.  Warps: slot 2 w + 1 where worker w begins a unit that others end, 2 w where it goes on with one. */
+static_assert((size_t)KV4_PARTS * (128 + 2) * sizeof(float) <= KV4_AREA_BYTES, "the tokens' partials");
 struct KaParts {
     float *max, *sum, *o; /* [slot][8 NT columns](, [128]) */
     unsigned* arrived;    /* [row][kv head] of a unit's first row */
@@ -745,7 +746,7 @@ static cudaError_t launch_attn(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
     }
     KaParts p;
     unsigned char* area = static_cast<unsigned char*>(c->work) + KV4_STATUS_BYTES;
-    p.arrived = reinterpret_cast<unsigned*>(area + kv4_area_bytes(c->n_pages));
+    p.arrived = reinterpret_cast<unsigned*>(area + KV4_AREA_BYTES);
     p.o = reinterpret_cast<float*>(area);
     p.max = p.o + (size_t)KV4_PARTS * 128;
     p.sum = p.max + KV4_PARTS;
@@ -762,8 +763,10 @@ extern "C" cudaError_t kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_b
         const cudaError_t e = kv4_slices(c, b, layer, few, q, out, st);
         if (e != cudaSuccess || !few) return e;
     }
-    /* next to slices most entries bring a single token, and those of a few rows read their sequence a few times */
-    return few < most || most * group <= 8 ? launch_attn<1>(c, b, layer, few, q, out, st) : launch_attn<2>(c, b, layer, few, q, out, st);
+    /* Next to slices most entries bring a single token, and those of a few rows read their sequence a few times.  A row's query heads of a kv
+     * head are not divided. */
+    const bool one = group <= 8 && (few < most || most * group <= 8);
+    return one ? launch_attn<1>(c, b, layer, few, q, out, st) : launch_attn<2>(c, b, layer, few, q, out, st);
 }
 
 }  // namespace s2p

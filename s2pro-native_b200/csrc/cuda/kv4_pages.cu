@@ -15,6 +15,7 @@ struct Kv4Lists {
     int2* moves;
     int* renumber;
 };
+static_assert(256 + ((size_t)KV4_MAX_PAGES / 2 + 1 + S2P_B200_KV4_MAX_LIST) * sizeof(int2) + (size_t)KV4_MAX_PAGES * sizeof(int) <= KV4_AREA_BYTES, "the lists");
 static inline Kv4Lists kv4_lists(const s2p_b200_kv4& c) {
     unsigned char* at = static_cast<unsigned char*>(c.work) + KV4_STATUS_BYTES;
     Kv4Lists l;

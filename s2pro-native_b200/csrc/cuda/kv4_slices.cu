@@ -107,7 +107,7 @@ __device__ __forceinline__ bool ks_wait(uint64_t* bar, unsigned parity, int* sta
     if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
     const unsigned long long t0 = pipe_now();
     for (unsigned i = 1; !mbar_try_wait(bar, parity); i++)
-        if ((i & 63u) == 0 && (status_peek(status) != PIPE_OK || pipe_now() - t0 > c_pipe_wait_ns || i >= PIPE_MBAR_TRIES)) {
+        if ((i & 7u) == 0 && (status_peek(status) != PIPE_OK || pipe_now() - t0 > c_pipe_wait_ns || i >= PIPE_MBAR_TRIES)) {
             atomicCAS(status, PIPE_OK, PIPE_ERR_TMA_WAIT);
             return false;
         }
@@ -145,6 +145,10 @@ __device__ __forceinline__ uint32_t ks_half2(float lo, float hi) {
 }
 __device__ __forceinline__ __half2 ks_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t ks_u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+/* Keys and values are held at half their size, so that the largest that the cache can stand for (65536) is an f16; scores and results are doubled
+ * where they are scaled anyway. */
+__device__ __forceinline__ uint32_t ks_halve(uint32_t w) { return ks_u(__hmul2(ks_h2(w), ks_h2(0x38003800u))); }
+__device__ __forceinline__ uint4 ks_halve(const uint4& w) { return make_uint4(ks_halve(w.x), ks_halve(w.y), ks_halve(w.z), ks_halve(w.w)); }
 /* eight codes of a word as s c + m: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7 (those of a byte's upper half come as 16 c) */
 __device__ __forceinline__ uint4 ks_widen(uint32_t w, __half2 s, __half2 m) {
     const __half2 k1024 = ks_h2(0x64006400u), k16th = ks_h2(0x2C002C00u), k64 = ks_h2(0xD400D400u); /* 1024, 1 / 16, -64 */
@@ -366,8 +370,8 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 const int largest = (int)max(big & 0xFFFFu, big >> 16), e = largest ? min(136 - (largest >> 7), 120) : 0; /* 2^9 <= it times 2^e < 2^10 */
                 const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                 if (r < KS_ROWS) {
-                    if (u == 0) /* log2(e) / sqrt(128) 2^-e */
-                        sh_factor[unit & 3][tile * KS_ROWS + r] = __uint_as_float((uint32_t)(127 - e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
+                    if (u == 0) /* 2 log2(e) / sqrt(128) 2^-e */
+                        sh_factor[unit & 3][tile * KS_ROWS + r] = __uint_as_float((uint32_t)(127 - e) << 23) * (2.0f * 1.4426950408889634f * 0.08838834764831845f);
                     uint4 h; /* channels 0, 4, 1, 5, 2, 6, 3, 7 of the unit of eight, as ks_widen puts them */
                     h.x = ks_half2(bf_lo(w[k].x) * up, bf_lo(w[k].z) * up);
                     h.y = ks_half2(bf_hi(w[k].x) * up, bf_hi(w[k].z) * up);
@@ -505,7 +509,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
 #pragma unroll
                     for (int k = 0; k < 32; k++) y[k] = __uint_as_float(v[k]);
                     if (whole) {
-                        if (live) store(c, y, sum == 0.0f ? 0.0f : 1.0f / sum);
+                        if (live) store(c, y, sum == 0.0f ? 0.0f : 2.0f / sum);
                     } else if (live) {
 #pragma unroll
                         for (int k = 0; k < 8; k++)
@@ -530,7 +534,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         bool ok = true;
         unsigned it = 0, segments = 0;
         int chunk = chunk_at;
-        for (unsigned cur = begin; cur < end && ok; segments++) {
+        for (unsigned cur = begin; cur < end; segments++) { /* (to its end whatever gave up: a team's warps meet at every page) */
             const Segment s = segment(cur, chunk);
             /* The queries of a unit go where the unit's before were as soon as its last scores are complete, while its last softmax and its result
              * are still to come; behind the team's first page of the unit, which waits for less. */
@@ -559,7 +563,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
 #pragma unroll
                     for (int j = 0; j < 2; j++) { /* this thread's units are in blocks p >> 6 and 2 + (p >> 6) */
                         const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
-                        const uint4 kc = *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16), kp = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16);
+                        const uint4 kc = *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16), kp = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16));
                         const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + g;
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
@@ -579,7 +583,8 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     for (int j = 0; j < 2; j++) {
                         const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
                         const uint4 vc = *reinterpret_cast<const uint4*>(blk + 1024 + plane * 512 + lane * 16);
-                        const uint4 vs = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16), vm = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16);
+                        const uint4 vs = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16)),
+                                    vm = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16));
                         const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + 2 * t;
 #pragma unroll
                         for (int k = 0; k < 4; k++) { /* positions pos, pos + 1; words of groups 0, 1 and 2, 3 */
@@ -738,7 +743,7 @@ __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int
         }
         top = now;
     }
-    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float scale = sum == 0.0f ? 0.0f : 2.0f / sum; /* (the values' halves) */
     __nv_bfloat16* to = out + ((size_t)(unit.x + row) * q_heads + unit.z * group + in % group) * 128 + 64 * (u >> 3) + 4 * (u & 7);
 #pragma unroll
     for (int odd = 0; odd < 2; odd++) {
@@ -754,6 +759,8 @@ static int ks_chunks(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b) {
     return most < (1 << 20) ? (int)most : 1 << 20;
 }
 constexpr int KS_MOST_SMEM = 221 * 1024; /* 227 KB less what is declared in the kernel */
+
+extern "C" cudaError_t kv4_slices_set_wait_ns(unsigned long long ns) { return cudaMemcpyToSymbol(c_pipe_wait_ns, &ns, sizeof(ns)); }
 
 extern "C" int kv4_slices_serve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b) {
     return KS_OPERANDS + ks_line_bytes(ks_chunks(c, b), b->n) <= (size_t)KS_MOST_SMEM;

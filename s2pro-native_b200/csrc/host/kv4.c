@@ -7,7 +7,7 @@
 static int misaligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
 
 static int sizes_served(const s2p_b200_kv4* c) {
-    return c && c->n_pages > 0 && c->layers > 0 && c->layers <= 1024 && c->kv_heads > 0 && c->kv_heads <= 1024 && c->q_heads > 0 &&
+    return c && c->n_pages > 0 && c->n_pages <= KV4_MAX_PAGES && c->layers > 0 && c->layers <= 1024 && c->kv_heads > 0 && c->kv_heads <= 1024 && c->q_heads > 0 &&
            c->q_heads % c->kv_heads == 0 && c->q_heads / c->kv_heads <= KV4_MAX_GROUP && c->max_seqs > 0 && c->table_stride > 0 &&
            c->table_stride <= KV4_MAX_STRIDE;
 }
@@ -18,13 +18,13 @@ size_t s2p_b200_kv4_page_bytes(int layers, int kv_heads) {
 }
 
 size_t s2p_b200_kv4_work_bytes(const s2p_b200_kv4* c, int rows) {
-    return !sizes_served(c) || rows < 0 ? 0 : kv4_work_bytes(c->n_pages, rows, c->kv_heads);
+    return !sizes_served(c) || rows < 0 ? 0 : kv4_work_bytes(rows, c->kv_heads);
 }
 
 static s2p_status check_cache(const char* what, const s2p_b200_kv4* c, int rows) {
     if (!sizes_served(c)) {
-        fprintf(stderr, "[s2pro] %s: the cache's sizes cannot be served (q_heads a multiple of kv_heads, at most %d times as many; up to %d table "
-                        "entries a sequence)\n", what, KV4_MAX_GROUP, KV4_MAX_STRIDE);
+        fprintf(stderr, "[s2pro] %s: the cache's sizes cannot be served (q_heads a multiple of kv_heads, at most %d times as many; up to %d pages, "
+                        "%d table entries a sequence)\n", what, KV4_MAX_GROUP, KV4_MAX_PAGES, KV4_MAX_STRIDE);
         return S2P_ERR_INVALID;
     }
     if (!c->pages || !c->table || !c->lens || !c->refs || !c->work) return S2P_ERR_INVALID;

@@ -59,7 +59,7 @@ def test_sizes(mine, capi):
     small, large = (mine.s2p_b200_kv4_work_bytes(C.byref(descriptor(capi, mine)), n) for n in (1, 100000))
     assert 0 < small < large
     for bad in (dict(q_heads=12), dict(q_heads=8 * 17), dict(kv_heads=0), dict(n_pages=0), dict(layers=0), dict(max_seqs=0), dict(table_stride=0),
-                dict(table_stride=(1 << 24) + 1)):
+                dict(table_stride=(1 << 24) + 1), dict(n_pages=(1 << 22) + 1)):
         assert mine.s2p_b200_kv4_work_bytes(C.byref(descriptor(capi, mine, **bad)), 1) == 0
     assert mine.s2p_b200_kv4_work_bytes(None, 1) == 0 and mine.s2p_b200_kv4_work_bytes(C.byref(descriptor(capi, mine)), -1) == 0
 
@@ -116,6 +116,11 @@ def test_row_calls_refuse_layers_and_pointers(mine, capi):
         assert mine.s2p_b200_kv4_attention(c, b, 0, x, y, None) == -1
         assert mine.s2p_b200_kv4_read(c, b, 0, x, y, None) == -1
     assert mine.s2p_b200_kv4_reserve(c, b, P + 2, None) == -1 and mine.s2p_b200_kv4_compact(c, P + 2, None) == -1
+
+
+def test_attention_refuses_more_work_than_it_counts(mine, capi):
+    c = C.byref(descriptor(capi, mine, table_stride=1 << 20))
+    assert mine.s2p_b200_kv4_attention(c, C.byref(batch(capi, rows=65)), 0, P, P, None) == -1
 
 
 def test_lists_are_checked(mine, capi):

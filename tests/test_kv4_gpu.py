@@ -139,6 +139,95 @@ def test_value_ranges(mine, capi, scale, rows):
     check_attention(cache, b, [(0, 330 - rows, 0, rows)], q, out)
 
 
+@pytest.mark.parametrize("rows", [1, 20, 150])
+def test_values_at_the_ends_of_f16(mine, capi, rows):
+    """Groups that stand for -65504 .. 65536: nothing on the way may leave f16.  (The bound of _kv4.attention holds relative to what is summed.)"""
+    cache = _kv4.Cache(mine, capi, 20, kv_heads=2, q_heads=8, stride=8, rows=rows)
+    _kv4.fill(cache, 0, 330, seed=5, scale=1e6)
+    assert float(cache.values(0, 330)[1].abs().max()) > 65504
+    b = cache.batch([0], [rows], [330 - rows])
+    q = queries(rows, 8, scale=1e-6)
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    check_attention(cache, b, [(0, 330 - rows, 0, rows)], q, out)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 33, 150])
+def test_out_may_be_the_queries(mine, capi, rows):
+    cache = _kv4.Cache(mine, capi, 40, kv_heads=2, q_heads=8, stride=32, rows=rows)
+    _kv4.fill(cache, 0, 1500, seed=5)
+    b = cache.batch([0], [rows], [1500 - rows])
+    q = queries(rows, 8)
+    out, both = torch.full_like(q, 7.0), q.clone()
+    cache.attention(b, q, out)
+    cache.attention(b, both, both)
+    torch.cuda.synchronize()
+    assert torch.equal(both, out)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(32, 8), (6, 2), (16, 1)])
+def test_many_slices(mine, capi, q_heads, kv_heads):
+    """More units than there are SMs, of all lengths: CTAs that end one unit, have others whole and begin a third; next to single tokens."""
+    import random
+    rng = random.Random(q_heads)
+    counts = [rng.choice((1, 2, 17, 40, 64, 65, 100, 128, 129, 200, 300)) for _ in range(14)]
+    firsts = [rng.choice((0, 1, 63, 64, 100, 500)) for _ in counts]
+    total = sum(counts)
+    cache = _kv4.Cache(mine, capi, 200, kv_heads=kv_heads, q_heads=q_heads, max_seqs=14, stride=16, rows=total)
+    for i, (p, n) in enumerate(zip(firsts, counts)):
+        _kv4.fill(cache, i, p + n, seed=i)
+    b = cache.batch(range(14), counts, firsts)
+    q = queries(total, q_heads)
+    outs = []
+    for _ in range(3):
+        out = torch.full_like(q, 7.0)
+        cache.attention(b, q, out)
+        outs.append(out)
+    at, entries = 0, []
+    for i, (p, n) in enumerate(zip(firsts, counts)):
+        entries.append((i, p, at, n))
+        at += n
+    check_attention(cache, b, entries, q, outs[0])
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    cache.call("status", None)
+
+
+def test_a_long_slice(mine, capi):
+    """CTAs that walk many pages of a unit, and units cut over many CTAs."""
+    cache = _kv4.Cache(mine, capi, 120, kv_heads=1, q_heads=4, max_seqs=1, stride=128, rows=700)
+    _kv4.fill(cache, 0, 7000, seed=3)
+    q = queries(700, 4)
+    for n in (700, 65):
+        b = cache.batch([0], [n], [7000 - n])
+        out = torch.full_like(q[:n], 7.0)
+        cache.attention(b, q[:n].contiguous(), out)
+        check_attention(cache, b, [(0, 7000 - n, 0, n)], q[:n], out)
+
+
+def test_as_many_sequences_as_a_batch_takes(mine, capi):
+    n = 1024
+    cache = _kv4.Cache(mine, capi, 1100, kv_heads=1, q_heads=2, max_seqs=n, stride=2, rows=n + 40)
+    cache.refs[:] = 0
+    book = [(i * 7) % 61 + 1 for i in range(n)]
+    b = cache.batch(range(n), book, max_rows=100)
+    cache.reserve(b)
+    torch.cuda.synchronize()
+    assert cache.info.cpu().tolist() == [1100 - n, 0] and cache.table[:, 0].cpu().tolist() == list(range(n))
+    for i in (0, 1, 511, 512, 1022, 1023):
+        _kv4.fill(cache, i, book[i], seed=i, order=torch.tensor([i]))
+    b = cache.batch(range(n), [1] * n, [t - 1 for t in book])
+    q = queries(n, 2)
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    check_attention(cache, b, [(i, book[i] - 1, i, 1) for i in (0, 1, 511, 512, 1022, 1023)], q, out)
+    b = cache.batch(range(n), [1] * 511 + [40] + [1] * 512, [max(0, t - 1) for t in book])  # one of them a slice
+    cache.pages[511:513] = 0
+    q = queries(n + 39, 2)
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    check_attention(cache, b, [(0, book[0] - 1, 0, 1), (1023, book[1023] - 1, n + 38, 1)], q, out)
+
+
 @pytest.mark.parametrize("rows", [1, 33])
 def test_queries_of_zero_and_of_extreme_size(mine, capi, rows):
     cache = _kv4.Cache(mine, capi, 20, kv_heads=1, q_heads=4, stride=8, rows=rows)
@@ -651,3 +740,72 @@ def test_a_captured_tick_replays_as_the_sequences_grow(mine, capi):
         torch.cuda.synchronize()
         assert torch.equal(b.pos0, b2.pos0) and torch.equal(q, q2) and torch.equal(out, out2)
     assert torch.equal(cache.table, again.table) and cache.lens.cpu().tolist() == [162, 101, 0, 230]
+
+
+def test_a_wait_that_gives_up_is_told_and_leaves_nothing_behind(testlib, capi):
+    """The deadline of the slices' bounded waits lowered until one runs out: the call ends, the status says so once, and with the deadline
+    restored the next call is right."""
+    capi.bind(testlib, capi.EXT_PROTOTYPES)
+    testlib.kv4_slices_set_wait_ns.argtypes = [C.c_ulonglong]
+    cache = _kv4.Cache(testlib, capi, 60, kv_heads=2, q_heads=8, max_seqs=2, stride=40, rows=400)
+    _kv4.fill(cache, 0, 2400, seed=1)
+    b = cache.batch([0], [400], [2000])
+    q = queries(400, 8)
+    out = torch.full_like(q, 7.0)
+    try:
+        assert testlib.kv4_slices_set_wait_ns(100) == 0
+        for _ in range(50):
+            cache.attention(b, q, out)
+            said = cache.status("status", None)
+            assert said in (0, -8)
+            if said:
+                break
+        assert said == -8
+    finally:
+        assert testlib.kv4_slices_set_wait_ns(2_000_000_000) == 0
+    cache.call("status", None)
+    cache.attention(b, q, out)
+    check_attention(cache, b, [(0, 2000, 0, 400)], q, out)
+    cache.call("status", None)
+
+
+def test_caches_share_a_workspace(mine, capi):
+    """Of other sizes, in turn."""
+    caches = [_kv4.Cache(mine, capi, n, kv_heads=h, q_heads=4 * h, stride=24, rows=300) for n, h in ((30, 2), (500, 8), (25, 1))]
+    for c in caches:
+        _kv4.fill(c, 0, 1400, seed=c.n_pages)
+        c.work = caches[1].work
+        c.c.work, c.c.work_bytes = c.work.data_ptr(), c.work.numel()
+    for turn in range(3):
+        for rows in (1, 20, 300):
+            for c in caches:
+                b = c.batch([0], [rows], [1400 - rows])
+                q = queries(rows, c.q_heads, seed=turn)
+                out = torch.full_like(q, 7.0)
+                c.attention(b, q, out)
+                check_attention(c, b, [(0, 1400 - rows, 0, rows)], q, out)
+                if turn == 1:
+                    c.compact()
+
+
+def test_two_streams_with_a_workspace_each(mine, capi):
+    """Two caches worked on at once."""
+    pairs = []
+    for i in range(2):
+        cache = _kv4.Cache(mine, capi, 60, kv_heads=2, q_heads=8, max_seqs=2, stride=40, rows=200)
+        _kv4.fill(cache, 0, 2000, seed=i)
+        pairs.append((cache, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = []
+    for turn in range(10):
+        for i, (cache, stream) in enumerate(pairs):
+            rows = (1, 200, 9)[(turn + i) % 3]
+            with torch.cuda.stream(stream):
+                b = cache.batch([0], [rows], [2000 - rows])
+                q = queries(rows, 8, seed=turn)
+                out = torch.full_like(q, 7.0)
+                cache.attention(b, q, out, stream=C.c_void_p(stream.cuda_stream))
+                outs.append((cache, b, rows, q, out))
+    torch.cuda.synchronize()
+    for cache, b, rows, q, out in outs:
+        check_attention(cache, b, [(0, 2000 - rows, 0, rows)], q, out)
