@@ -392,7 +392,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
         const int rows = batch.start[e + 1] - batch.start[e];
         return rows > few || !rows ? 0 : rows <= rows_per ? cache.kv_heads : (rows + rows_per - 1) / rows_per * cache.kv_heads;
     };
-    /* Brought by all, worked out by one warp, 32 entries at a time: two barriers.  (By all warps, with a barrier for every sum, 0.6 us more.) */
+    /* Brought by all, worked out by one warp, 128 entries at a time: two barriers.  (By all warps, with a barrier for every sum, 0.6 us more.) */
     for (int e = tid; e <= b.n; e += KA_THREADS) {
         const int r = b.row0[e];
         if (e < b.n) {
@@ -416,40 +416,61 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
             return mine;
         };
         int top = 0;
-        for (int e0 = 0; e0 <= b.n; e0 += 32) {
-            const int e = e0 + lane;
-            int r = max(e <= b.n ? batch.start[e] : 0, top);
+        for (int e0 = 0; e0 <= b.n; e0 += 128) {
+            int r[4], run = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = e0 + 4 * lane + i;
+                if (e <= b.n) run = max(run, batch.start[e]);
+                r[i] = run;
+            }
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
-                const int o = __shfl_up_sync(S2P_FULL_MASK, r, off);
-                if (lane >= off) r = max(r, o);
+                const int o = __shfl_up_sync(S2P_FULL_MASK, run, off);
+                if (lane >= off) run = max(run, o);
             }
-            if (e <= b.n) batch.start[e] = r;
-            top = __shfl_sync(S2P_FULL_MASK, r, 31);
+            const int left = __shfl_up_sync(S2P_FULL_MASK, run, 1), base = max(top, lane ? left : 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e0 + 4 * lane + i <= b.n) batch.start[e0 + 4 * lane + i] = max(r[i], base);
+            top = max(top, __shfl_sync(S2P_FULL_MASK, run, 31));
         }
         __syncwarp();
-        unsigned total = 0, units = 0;
-        for (int e0 = 0; e0 <= b.n; e0 += 32) {
-            const int e = e0 + lane;
-            const unsigned u = e < b.n ? (unsigned)units_of(e) : 0u;
-            units += __reduce_add_sync(S2P_FULL_MASK, u);
-            const unsigned at = before(u ? u * (unsigned)blocks_of(e) : 0u, total);
-            if (e <= b.n) batch.upto[e] = at;
-        }
+        /* upto[e] = the sum of what `of` gives for the entries before e; all of it */
+        auto line_up = [&](auto of) {
+            unsigned all = 0;
+            for (int e0 = 0; e0 <= b.n; e0 += 128) {
+                unsigned v[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = e0 + 4 * lane + i;
+                    v[i] = e < b.n ? of(e) : 0u;
+                    sum += v[i];
+                }
+                unsigned at = before(sum, all);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = e0 + 4 * lane + i;
+                    if (e <= b.n) batch.upto[e] = at;
+                    at += v[i];
+                }
+            }
+            return all;
+        };
+        unsigned units = 0;
+        const unsigned total = line_up([&](int e) {
+            const unsigned u = (unsigned)units_of(e);
+            units += u;
+            return u * (unsigned)blocks_of(e);
+        });
+        units = __reduce_add_sync(S2P_FULL_MASK, units);
         /* Few units on short sequences: each is cut into parts, a CTA to a part, its warps a stretch of it each.  Otherwise warps work by
          * themselves (no barriers, but a partial for every warp) on equal stretches of the line of all units' blocks. */
         const bool by_warp = total >= gridDim.x * KA_WARPS * KA_LONG || 2 * units > gridDim.x;
         unsigned workers = min(gridDim.x * KA_WARPS, (total + KA_LEAST_WARP - 1) / KA_LEAST_WARP), longest = 1;
         if (!by_warp) {
             longest = max((unsigned)KA_LEAST_CTA, (total + gridDim.x - units - 1) / (gridDim.x - units)); /* so there are at most gridDim.x parts */
-            workers = 0;
-            __syncwarp();
-            for (int e0 = 0; e0 <= b.n; e0 += 32) {
-                const int e = e0 + lane;
-                const unsigned u = e < b.n ? (unsigned)units_of(e) : 0u;
-                const unsigned at = before(u ? u * ((blocks_of(e) + longest - 1) / longest) : 0u, workers);
-                if (e <= b.n) batch.upto[e] = at;
-            }
+            workers = line_up([&](int e) { return (unsigned)units_of(e) * ((blocks_of(e) + longest - 1) / longest); });
         }
         if (lane == 0) {
             sh_line.by_warp = by_warp;
