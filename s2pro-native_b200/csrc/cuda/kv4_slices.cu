@@ -19,9 +19,12 @@
  * core-matrix layout (8 rows x 16 bytes); a unit plane has 32 or 16 bytes more than its positions take, so that the converting lanes'
  * stores fall on different banks.
  *
- * Work is cut like that of single tokens: the pages of all units form one line, each CTA takes an equal stretch of it.  The parts of a
- * shared unit are added, in order, by a second kernel over all SMs: in the last CTA to arrive that took 8 us for two parts of 128 KB and
- * 20 for five, with the other SMs idle. */
+ * The pages of all units form one line, and each CTA takes an equal stretch of it, wherever that cuts units.  With no more units than CTAs
+ * most CTAs would get the end of one unit and the start of the next: there every unit is cut into equal parts of its own, one to a CTA
+ * (32 query and 8 kv heads, 512 rows behind 1500: 49 -> 41 us, 77 rows behind 100: 30 -> 24.5).  The parts of a
+ * unit are added, in order, by a second kernel over all SMs: in the last CTA to arrive that took 8 us for two parts of 128 KB and 20 for
+ * five, with the other SMs idle.  Parts stay in 32 bits (f16 would take 1.5 us off the smallest calls).
+ * A page takes a CTA 1.25 us; the tensor cores are busy 54% of that, the rest is the softmax's and the converters' instructions. */
 #include "kv4.cuh"
 #include "pipe.cuh"
 
@@ -32,7 +35,8 @@ constexpr int KS_Q_PITCH = 128 * 16 + 16, KS_Q_BYTES = 16 * KS_Q_PITCH;         
 constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
 constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + 2 * KS_RAW * KV4_HEAD_BYTES;
-constexpr int KS_LEAST = 2;                                                /* pages that make a CTA worth its while */
+constexpr int KS_LEAST = 3;  /* pages that make a CTA worth its while: 77 rows behind 100 with 2 and 3: 26.9 and 25.2 us; longer calls have more in any case */
+constexpr int KS_SECOND = 4; /* pages that a second unit costs a CTA (5 us: queries, a part to write, another's to read) */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
 struct KsBars {
@@ -169,6 +173,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     __shared__ KsBars bars;
     __shared__ uint32_t sh_tmem;
     __shared__ float sh_factor[4][KS_SOFTMAX]; /* of the query rows of a unit, four units deep: to base-2 logits */
+    __shared__ struct { unsigned begin, end, last, share, more; } sh_line; /* this CTA's stretch; the last CTA of the one unit it has a part of, or 0; all stretches */
     __shared__ int sh_absent[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = cache.q_heads / cache.kv_heads, tile_rows = KS_ROWS / group, unit_rows = 2 * tile_rows;
@@ -264,24 +269,67 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             if (e <= b.n) line.first[e] = (int)at;
         }
         __syncwarp();
+        int most = 0; /* pages of the longest unit */
         for (int c0 = 0; c0 <= (int)chunks; c0 += 32) {
             const int c = c0 + lane;
-            const unsigned at = before(c < (int)chunks ? (unsigned)tiles_of(entry_of(c), c) * (unsigned)cache.kv_heads : 0u, total);
+            const int t = c < (int)chunks ? tiles_of(entry_of(c), c) : 0;
+            most = max(most, t);
+            const unsigned at = before((unsigned)t * (unsigned)cache.kv_heads, total);
             if (c <= (int)chunks) line.upto[c] = at;
+        }
+        most = (int)__reduce_max_sync(S2P_FULL_MASK, (unsigned)most);
+        __syncwarp();
+        /* As many units as CTAs or fewer: each is cut into parts of at most `longest` pages, the shortest for which there is a CTA to each part; unless a
+         * CTA's equal share of the line is shorter by more than a second unit costs it (its queries, its part, and the other's reading of it). */
+        const unsigned heads = (unsigned)cache.kv_heads;
+        unsigned workers = min(gridDim.x, (total + KS_LEAST - 1) / KS_LEAST), longest = 0;
+        if (chunks * heads <= gridDim.x && chunks) {
+            auto parts_at = [&](unsigned l) {
+                unsigned n = 0;
+                for (int c = lane; c < (int)chunks; c += 32) n += ((line.upto[c + 1] - line.upto[c]) / heads + l - 1) / l;
+                return __reduce_add_sync(S2P_FULL_MASK, n) * heads;
+            };
+            unsigned lo = KS_LEAST, hi = max((unsigned)most, (unsigned)KS_LEAST);
+            while (lo < hi) {
+                const unsigned mid = (lo + hi) / 2;
+                if (parts_at(mid) <= gridDim.x) hi = mid;
+                else lo = mid + 1;
+            }
+            if (lo <= total / gridDim.x + KS_SECOND) {
+                longest = lo;
+                workers = 0;
+                if (lane == 0) sh_line.begin = sh_line.end = 0;
+                __syncwarp();
+                for (int c0 = 0; c0 < (int)chunks; c0 += 32) {
+                    const int c = c0 + lane;
+                    const unsigned t = c < (int)chunks ? (line.upto[c + 1] - line.upto[c]) / heads : 0u, cuts = (t + longest - 1) / longest;
+                    const unsigned at = before(cuts * heads, workers);
+                    if (blockIdx.x >= at && blockIdx.x - at < cuts * heads) {
+                        const unsigned head = (blockIdx.x - at) / cuts, cut = blockIdx.x - at - head * cuts, each = t / cuts, over = t - each * cuts;
+                        sh_line.begin = line.upto[c] + head * t + each * cut + min(cut, over);
+                        sh_line.end = sh_line.begin + each + (cut < over);
+                        sh_line.last = blockIdx.x - cut + cuts - 1;
+                    }
+                }
+            }
+        }
+        if (lane == 0 && !longest) {
+            const unsigned share = workers ? total / workers : 1, more = workers ? total - share * workers : 0, w = min(blockIdx.x, workers);
+            sh_line.begin = share * w + min(w, more);
+            sh_line.end = blockIdx.x < workers ? sh_line.begin + share + (w < more) : sh_line.begin;
+            sh_line.last = 0;
+            sh_line.share = share;
+            sh_line.more = more;
         }
     }
     __syncthreads();
     ks_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh_tmem);
-    const unsigned chunks = (unsigned)line.first[b.n], total = line.upto[chunks];
-    const unsigned workers = min(gridDim.x, (total + KS_LEAST - 1) / KS_LEAST);
-    const unsigned share = workers ? total / workers : 1, more = workers ? total - share * workers : 0, worker = blockIdx.x;
-    const unsigned begin = worker < workers ? share * worker + min(worker, more) : 0, end = worker < workers ? begin + share + (worker < more) : 0;
-    auto worker_of = [&](unsigned x) { return x < (share + 1) * more ? x / (share + 1) : more + (x - (share + 1) * more) / share; };
+    const unsigned chunks = (unsigned)line.first[b.n], worker = blockIdx.x;
+    const unsigned begin = sh_line.begin, end = sh_line.end;
 
     struct Segment {
-        int e, head, row0, n_rows, seq, p0, seen, t0, t1, tiles, r0;
-        unsigned u0;
+        int e, head, row0, n_rows, seq, p0, seen, t0, t1, tiles, r0; /* pages t0 .. t1 - 1 of `tiles` */
     };
     int chunk_at = 0;
     if (begin < end) {
@@ -292,6 +340,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         }
         chunk_at = lo;
     }
+    auto last_of = [&](const Segment& s, unsigned cur) { /* the last CTA of the unit that this one begins */
+        if (sh_line.last) return sh_line.last;
+        const unsigned x = cur + (unsigned)s.tiles - 1, longer = (sh_line.share + 1) * sh_line.more;
+        return x < longer ? x / (sh_line.share + 1) : sh_line.more + (x - longer) / sh_line.share;
+    };
     auto segment = [&](unsigned cur, int& chunk) {
         Segment s;
         while (line.upto[chunk + 1] <= cur) chunk++;
@@ -301,7 +354,6 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         s.head = (int)(inside / (unsigned)s.tiles);
         s.t0 = (int)(inside - (unsigned)s.head * (unsigned)s.tiles);
         s.t1 = s.t0 + (int)min((unsigned)(s.tiles - s.t0), end - cur);
-        s.u0 = cur - (unsigned)s.t0;
         s.r0 = (chunk - line.first[s.e]) * unit_rows;
         s.n_rows = min(unit_rows, rows_of(s.e) - s.r0);
         s.row0 = line.start[s.e] + s.r0;
@@ -482,7 +534,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             if (!ok) break; /* the other warps' waits give up by themselves: the status word is set */
 
             const bool whole = s.t0 == 0 && s.t1 == s.tiles;
-            auto store = [&](int c, const float (&v)[32], float scale) { /* columns 32 c ..: units 4 c .. 4 c + 3 of values, two groups in turn */
+            auto store = [&](int c, const float (&v)[32]) { /* columns 32 c ..: units 4 c .. 4 c + 3 of values, two groups in turn */
                 __nv_bfloat16* to = out + at + 64 * (c >> 1) + 16 * (c & 1);
 #pragma unroll
                 for (int odd = 0; odd < 2; odd++)
@@ -492,7 +544,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int at0 = 16 * h + 4 * k + odd; /* unit 2 h + k / 2, channels 2 (k % 2), + 1 */
-                            const __nv_bfloat162 y = __floats2bfloat162_rn(v[at0] * scale, v[at0 + 2] * scale);
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(v[at0], v[at0 + 2]);
                             w[k] = *reinterpret_cast<const uint32_t*>(&y);
                         }
                         *reinterpret_cast<uint4*>(to + 32 * odd + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -506,14 +558,14 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     ks_ld32(t_o + 32 * c, v);
                     ks_ld_wait();
                     float y[32];
+                    const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 2.0f / sum; /* (the values' halves) */
 #pragma unroll
-                    for (int k = 0; k < 32; k++) y[k] = __uint_as_float(v[k]);
+                    for (int k = 0; k < 32; k++) y[k] = __uint_as_float(v[k]) * scale;
                     if (whole) {
-                        if (live) store(c, y, sum == 0.0f ? 0.0f : 2.0f / sum);
+                        if (live) store(c, y);
                     } else if (live) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            parts.o[(slot * 32 + 8 * c + k) * KS_SOFTMAX + tid] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                        for (int k = 0; k < 8; k++) parts.o[(slot * 32 + 8 * c + k) * KS_SOFTMAX + tid] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
                     }
                 }
                 ks_before_sync(); /* the next unit's first product writes where this has been read */
@@ -522,7 +574,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     parts.sum[slot * KS_SOFTMAX + tid] = sum;
                 }
             }
-            if (tid == 0 && s.t0 == 0 && !whole) parts.unit[worker] = make_int4(s.row0, s.n_rows, s.head, (int)worker_of(s.u0 + (unsigned)s.tiles - 1));
+            if (tid == 0 && s.t0 == 0 && !whole) parts.unit[worker] = make_int4(s.row0, s.n_rows, s.head, (int)last_of(s, cur));
             begun |= s.t0 == 0 && !whole;
             cur += (unsigned)(s.t1 - s.t0);
         }
@@ -673,7 +725,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     turn = next_turn;
                 }
                 if (ok) ks_commit(&bars.unit_done);
-                cur += (unsigned)tiles;
+                cur += (unsigned)(s.t1 - s.t0);
             }
             /* TMEM must not be freed under products in flight: they complete by themselves, and this waits for them with a limit of its own */
             ks_commit(&bars.all_done[x]);
@@ -695,7 +747,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
 
 /* The parts of shared units, in order of the CTAs that left them.  Block (w, y): 32 rows of the unit that CTA w began; a thread has one unit of eight
  * columns of a row, and eight parts' loads are under way at a time. */
-constexpr int KS_JOIN_ROWS = 32, KS_JOIN_THREADS = 16 * KS_JOIN_ROWS, KS_JOIN_PARTS = 8;
+constexpr int KS_JOIN_ROWS = 32, KS_JOIN_THREADS = 16 * KS_JOIN_ROWS, KS_JOIN_PARTS = 4;
 __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int q_heads, int group, __nv_bfloat16* out) {
     grid_wait();
     grid_release();
@@ -711,34 +763,35 @@ __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int
         float m[KS_JOIN_PARTS], l[KS_JOIN_PARTS];
         float4 v[KS_JOIN_PARTS][2];
 #pragma unroll
-        for (int i = 0; i < KS_JOIN_PARTS; i++) { /* (past the last part: its own again, with no weight) */
-            const int at = min(w + i, w1);
-            const size_t slot = (size_t)(2 * at + (at == w0));
-            m[i] = __ldcg(parts.max + slot * KS_SOFTMAX + r);
-            l[i] = __ldcg(parts.sum + slot * KS_SOFTMAX + r);
-            v[i][0] = __ldcg(parts.o + (slot * 32 + 2 * u) * KS_SOFTMAX + r);
-            v[i][1] = __ldcg(parts.o + (slot * 32 + 2 * u + 1) * KS_SOFTMAX + r);
+        for (int i = 0; i < KS_JOIN_PARTS; i++) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+            v[i][0] = v[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (w + i <= w1) {
+                const size_t slot = (size_t)(2 * (w + i) + (w + i == w0));
+                m[i] = __ldcg(parts.max + slot * KS_SOFTMAX + r);
+                l[i] = __ldcg(parts.sum + slot * KS_SOFTMAX + r);
+                v[i][0] = __ldcg(parts.o + (slot * 32 + 2 * u) * KS_SOFTMAX + r);
+                v[i][1] = __ldcg(parts.o + (slot * 32 + 2 * u + 1) * KS_SOFTMAX + r);
+            }
         }
         float now = top;
 #pragma unroll
-        for (int i = 0; i < KS_JOIN_PARTS; i++) {
-            if (w + i > w1) m[i] = -INFINITY;
-            now = fmaxf(now, m[i]);
-        }
+        for (int i = 0; i < KS_JOIN_PARTS; i++) now = fmaxf(now, m[i]);
         const float base = now == -INFINITY ? 0.0f : now, keep = ks_exp2(top - base);
         sum *= keep;
 #pragma unroll
         for (int k = 0; k < 8; k++) y[k] *= keep;
 #pragma unroll
         for (int i = 0; i < KS_JOIN_PARTS; i++) {
-            const float scale = ks_exp2(m[i] - base);
-            sum = fmaf(l[i], scale, sum);
+            const float weight = ks_exp2(m[i] - base);
+            sum = fmaf(l[i], weight, sum);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                y[4 * k] = fmaf(v[i][k].x, scale, y[4 * k]);
-                y[4 * k + 1] = fmaf(v[i][k].y, scale, y[4 * k + 1]);
-                y[4 * k + 2] = fmaf(v[i][k].z, scale, y[4 * k + 2]);
-                y[4 * k + 3] = fmaf(v[i][k].w, scale, y[4 * k + 3]);
+                y[4 * k] = fmaf(v[i][k].x, weight, y[4 * k]);
+                y[4 * k + 1] = fmaf(v[i][k].y, weight, y[4 * k + 1]);
+                y[4 * k + 2] = fmaf(v[i][k].z, weight, y[4 * k + 2]);
+                y[4 * k + 3] = fmaf(v[i][k].w, weight, y[4 * k + 3]);
             }
         }
         top = now;
