@@ -17,10 +17,9 @@
  *   values   O^T [128 channels x columns]: A = values, the pairs of positions put together by byte permutation, B = p^T, which is
  *            S^T transposed in registers (movmatrix), times s of the group (rounded to f16 once more; at most 4 * 8734).
  *
- * The cache is read once, so what bounds single tokens is HBM.  Work is cut evenly: the blocks of all units form one line, each
- * CTA takes an equal stretch of it, its warps the stretch's blocks in turn through a ring of asynchronous copies of their own; a
- * unit that several CTAs share is put together by the last of them to arrive, in the CTAs' order, so that the result does not
- * depend on timing. */
+ * The cache is read once, so what bounds single tokens is HBM.  A CTA or a warp takes an equal part of a unit, or an equal stretch of the
+ * line of all units' blocks; a warp walks its blocks through a ring of asynchronous copies of its own.  A unit that several share is put
+ * together by the last of them to arrive, in their order, so that the result does not depend on timing. */
 #include <limits.h>
 #include "kv4.cuh"
 #include "pipe.cuh"
@@ -31,12 +30,18 @@ constexpr int KA_WARPS = 8, KA_THREADS = KA_WARPS * 32, KA_PIECE = 4, KA_STAGES 
 constexpr int KA_RING_BYTES = KA_WARPS * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
 constexpr int KA_PASS = 4;                                         /* columns merged at a time */
 constexpr int KA_MERGE_BYTES = KA_WARPS * KA_PASS * 128 * 4;
-constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 4;           /* blocks that make a worker worth its while */
+constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 8;          /* blocks that make a worker worth its while */
 /* (Row, head) columns of a kv head up to which an entry is this kernel's rather than that of the tensor cores: alone, and next to longer slices, where
  * most bring a token.  us here and there, 32 / 8 heads: 4, 16, 32, 64 rows of one sequence at 1100 positions 16.9, 18.2, 19.5, 42 and 16.4, 18.1,
  * 20.3, 24.6; at 8000 positions 19.9, 27.6, 52, 61 and 27.9, 29.3, 33.4, 41.8; 4, 8, 16 rows of 16 sequences at 4000 53, 57, 82 and 72, 73, 75. */
 constexpr int KA_FEW = 64, KA_FEW_BESIDE = 32;
-constexpr int KA_LONG = 20;                                        /* blocks of a warp from which on warps work by themselves */
+/* How the work is cut (us, 32 query and 8 kv heads, one row a sequence).  Units each cut into equal parts, one to a CTA, its warps joined through shared memory,
+ * wherever there are no more units than CTAs: 15 sequences of 1500 13.0, by warps below 20.6; up to KA_LONG blocks to a warp, where the warps' barriers cost more
+ * than the partials that they save (9 of 8000 28.2 and 27.5, 12 of 4000 24.0 and 22.8), and where no part has KA_SECOND blocks more than an equal share (one
+ * sequence of 2000 among 15 of 1000, 67 more: 14.6 and 16.4; of 3000, 130 more: 18.2 and 17.8).  Otherwise a warp is a worker by itself and leaves a partial.
+ * Equal parts of each unit again (64 of 512: 18.0, 24 of 2500: 23.5), unless a part has KA_SECOND_WARP blocks more than an equal stretch of the line of all units'
+ * blocks, in which many warps end one unit and begin the next (64 of 512 20.5, 24 of 2500 26.2; but 32 of 8192, 18 more: 58.5, in parts 66). */
+constexpr int KA_SECOND = 120, KA_SECOND_WARP = 8, KA_LONG = 20;
 
 struct KaBatch { /* in shared memory, [n (+ 1)] */
     unsigned* upto;  /* blocks of all units before entry e */
@@ -306,17 +311,17 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
     }
 }
 
-/* Partial results.  CTAs: slot w for part w.  Warps: slot 2 w + 1 where worker w begins a unit that others end, 2 w where it goes on with one. */
+/* Partial results: slot 2 w + 1 where worker w begins a unit that others end, 2 w where it goes on with one. */
 static_assert((size_t)KV4_PARTS * (128 + 2) * sizeof(float) <= KV4_AREA_BYTES, "the tokens' partials");
 struct KaParts {
     float *max, *sum, *o; /* [slot][8 NT columns](, [128]) */
     unsigned* arrived;    /* [row][kv head] of a unit's first row */
 };
 
-/* What the workers from, from + step, ... up to `last` left of a unit (per: slots of a worker; starts: the warp that begins it), for columns base .. base + 3: running
+/* What the workers from, from + step, ... up to `last` left of a unit (starts: the one that begins it), for columns base .. base + 3: running
  * maximum, sum, and channels 4 lane .. 4 lane + 3 of the weighted values.  Sixteen loads are under way at a time. */
 template <int COLS>
-__device__ __forceinline__ void ka_gather(const KaParts& parts, int per, int starts, int from, int step, int last, int base, int columns, int lane, float (&top)[KA_PASS],
+__device__ __forceinline__ void ka_gather(const KaParts& parts, int starts, int from, int step, int last, int base, int columns, int lane, float (&top)[KA_PASS],
                                           float (&sum)[KA_PASS], float4 (&acc)[KA_PASS]) {
 #pragma unroll
     for (int k = 0; k < KA_PASS; k++) {
@@ -330,7 +335,7 @@ __device__ __forceinline__ void ka_gather(const KaParts& parts, int per, int sta
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int w = w0 + i * step;
-            const size_t at = (size_t)(per * w + (w == starts)) * COLS + base;
+            const size_t at = (size_t)(2 * w + (w == starts)) * COLS + base;
 #pragma unroll
             for (int k = 0; k < KA_PASS; k++) {
                 const bool there = w <= last && base + k < columns;
@@ -371,7 +376,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
     constexpr int COLS = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sh_max[KA_WARPS][COLS], sh_sum[KA_WARPS][COLS];
-    __shared__ struct { unsigned by_warp, workers, longest, share, more; } sh_line;
+    __shared__ struct { unsigned by_warp, cut, workers, share, more; } sh_line;
     __shared__ int sh_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem + warp * KA_STAGES * KA_PIECE * KV4_BLOCK_BYTES;
@@ -403,18 +408,18 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
         batch.start[e] = min(r, b.rows);
     }
     __syncthreads();
-    if (warp == 0) {
-        auto before = [&](unsigned v, unsigned& carry) { /* carry + the lanes before this one; carry goes on */
-            unsigned at = v;
+    auto before = [&](unsigned v, unsigned& carry) { /* carry + the lanes before this one; carry goes on */
+        unsigned at = v;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
-                if (lane >= off) at += o;
-            }
-            const unsigned mine = carry + at - v;
-            carry += __shfl_sync(S2P_FULL_MASK, at, 31);
-            return mine;
-        };
+        for (int off = 1; off < 32; off <<= 1) {
+            const unsigned o = __shfl_up_sync(S2P_FULL_MASK, at, off);
+            if (lane >= off) at += o;
+        }
+        const unsigned mine = carry + at - v;
+        carry += __shfl_sync(S2P_FULL_MASK, at, 31);
+        return mine;
+    };
+    if (warp == 0) {
         int top = 0;
         for (int e0 = 0; e0 <= b.n; e0 += 128) {
             int r[4], run = 0;
@@ -436,68 +441,84 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
             top = max(top, __shfl_sync(S2P_FULL_MASK, run, 31));
         }
         __syncwarp();
-        /* upto[e] = the sum of what `of` gives for the entries before e; all of it */
-        auto line_up = [&](auto of) {
-            unsigned all = 0;
-            for (int e0 = 0; e0 <= b.n; e0 += 128) {
-                unsigned v[4], sum = 0;
+        /* upto[e] = the blocks of the entries before e */
+        unsigned units = 0, total = 0, most = 0;
+        for (int e0 = 0; e0 <= b.n; e0 += 128) {
+            unsigned v[4], sum = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int e = e0 + 4 * lane + i;
-                    v[i] = e < b.n ? of(e) : 0u;
-                    sum += v[i];
-                }
-                unsigned at = before(sum, all);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int e = e0 + 4 * lane + i;
-                    if (e <= b.n) batch.upto[e] = at;
-                    at += v[i];
-                }
+            for (int i = 0; i < 4; i++) {
+                const int e = e0 + 4 * lane + i;
+                const unsigned u = e < b.n ? (unsigned)units_of(e) : 0u, l = u ? (unsigned)blocks_of(e) : 0u;
+                units += u;
+                most = max(most, l);
+                v[i] = u * l;
+                sum += v[i];
             }
-            return all;
-        };
-        unsigned units = 0;
-        const unsigned total = line_up([&](int e) {
-            const unsigned u = (unsigned)units_of(e);
-            units += u;
-            return u * (unsigned)blocks_of(e);
-        });
+            unsigned at = before(sum, total);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = e0 + 4 * lane + i;
+                if (e <= b.n) batch.upto[e] = at;
+                at += v[i];
+            }
+        }
         units = __reduce_add_sync(S2P_FULL_MASK, units);
-        /* Few units on short sequences: each is cut into parts, a CTA to a part, its warps a stretch of it each.  Otherwise warps work by
-         * themselves (no barriers, but a partial for every warp) on equal stretches of the line of all units' blocks. */
-        const bool by_warp = total >= gridDim.x * KA_WARPS * KA_LONG || 2 * units > gridDim.x;
-        unsigned workers = min(gridDim.x * KA_WARPS, (total + KA_LEAST_WARP - 1) / KA_LEAST_WARP), longest = 1;
-        if (!by_warp) {
-            longest = max((unsigned)KA_LEAST_CTA, (total + gridDim.x - units - 1) / (gridDim.x - units)); /* so there are at most gridDim.x parts */
-            workers = line_up([&](int e) { return (unsigned)units_of(e) * ((blocks_of(e) + longest - 1) / longest); });
+        most = __reduce_max_sync(S2P_FULL_MASK, most);
+        const unsigned grid = gridDim.x, warps = grid * KA_WARPS;
+        /* parts of at most this many blocks are no more than there are workers; the longest of those parts */
+        auto cut_for = [&](unsigned workers, unsigned least) { return max(least, (total + workers - units - 1) / (workers - units)); };
+        auto part_of = [&](unsigned cut) { return cut ? (most + (most + cut - 1) / cut - 1) / max(1u, (most + cut - 1) / cut) : 0u; };
+        unsigned cut = units < grid && total < warps * KA_LONG ? cut_for(grid, KA_LEAST_CTA) : 0;
+        bool by_warp = !cut || part_of(cut) > total / grid + KA_SECOND;
+        if (by_warp) {
+            cut = units < warps ? cut_for(warps, KA_LEAST_WARP) : 0;
+            if (part_of(cut) > total / warps + KA_SECOND_WARP) cut = 0;
         }
         if (lane == 0) {
+            const unsigned workers = min(warps, (total + KA_LEAST_WARP - 1) / KA_LEAST_WARP);
             sh_line.by_warp = by_warp;
-            sh_line.workers = workers;
-            sh_line.longest = longest;
+            sh_line.cut = cut;
             /* worker w of the line has `share` blocks, the first `more` workers one more */
-            sh_line.share = by_warp && workers ? total / workers : 1;
-            sh_line.more = by_warp ? total - sh_line.share * workers : 0;
+            sh_line.workers = workers;
+            sh_line.share = workers ? total / workers : 1;
+            sh_line.more = workers ? total - sh_line.share * workers : 0;
         }
     }
     __syncthreads();
     const bool by_warp = sh_line.by_warp;
-    const unsigned workers = sh_line.workers, longest = sh_line.longest, share = sh_line.share, more = sh_line.more;
-    const unsigned worker = by_warp ? warp * gridDim.x + blockIdx.x : blockIdx.x;
-    if (worker >= workers) return;
-    const unsigned begin = by_warp ? share * worker + min(worker, more) : worker, end = by_warp ? begin + share + (worker < more) : begin + 1;
-    auto worker_of = [&](unsigned x) { return x < (share + 1) * more ? x / (share + 1) : more + (x - (share + 1) * more) / share; };
-
-    int e = 0;
-    { /* the last entry that begins at or before `begin` */
+    const unsigned share = sh_line.share, more = sh_line.more, worker = by_warp ? warp * gridDim.x + blockIdx.x : blockIdx.x;
+    unsigned begin = 0, end = 0;
+    int e = 0, w_first = -1, w_last = -1; /* the entry; of a unit in parts: its workers */
+    if (const unsigned longest = sh_line.cut) {
+        unsigned carry = 0;
+        for (int e0 = 0; e0 < b.n && carry <= worker; e0 += 32) {
+            const int mine = e0 + lane;
+            const unsigned u = mine < b.n ? (unsigned)units_of(mine) : 0u, l = u ? (unsigned)blocks_of(mine) : 0u, cuts = (l + longest - 1) / longest;
+            const unsigned at = before(u * cuts, carry), found = __ballot_sync(S2P_FULL_MASK, worker >= at && worker - at < u * cuts);
+            if (found) {
+                const int who = __ffs(found) - 1;
+                const unsigned in = worker - __shfl_sync(S2P_FULL_MASK, at, who), n = __shfl_sync(S2P_FULL_MASK, cuts, who), blocks = __shfl_sync(S2P_FULL_MASK, l, who);
+                const unsigned unit = in / n, c = in - unit * n, piece = blocks / n, rest = blocks - piece * n;
+                e = e0 + who;
+                begin = batch.upto[e] + unit * blocks + piece * c + min(c, rest);
+                end = begin + piece + (c < rest);
+                w_first = (int)(worker - c);
+                w_last = w_first + (int)n - 1;
+            }
+        }
+    } else if (worker < sh_line.workers) {
+        begin = share * worker + min(worker, more);
+        end = begin + share + (worker < more);
         int lo = 0, hi = b.n;
-        while (hi - lo > 1) {
+        while (hi - lo > 1) { /* the last entry that begins at or before `begin` */
             const int mid = (lo + hi) >> 1;
             if (batch.upto[mid] <= begin) lo = mid; else hi = mid;
         }
         e = lo;
     }
+    if (begin == end) return;
+    auto worker_of = [&](unsigned x) { return x < (share + 1) * more ? x / (share + 1) : more + (x - (share + 1) * more) / share; };
+
     struct Segment { /* the stretch's part in one unit */
         int row, n_rows, r0, head, seq, p0, seen, least, blocks, x0, x1, w0, w1; /* blocks x0 .. x1 - 1 of `blocks`; the workers of the unit */
         int xa, xb, pieces;                                                    /* this warp's blocks, in pieces that end where a page does */
@@ -508,23 +529,14 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
         const int rows = batch.start[e + 1] - batch.start[e];
         s.blocks = blocks_of(e);
         const unsigned inside = cur - batch.upto[e];
-        unsigned unit;
-        if (by_warp) {
-            unit = inside / (unsigned)s.blocks;
-            s.x0 = (int)(inside - unit * (unsigned)s.blocks);
-            s.x1 = s.x0 + (int)min((unsigned)(s.blocks - s.x0), end - cur);
-            s.w0 = (int)worker_of(cur - (unsigned)s.x0);
-            s.w1 = (int)worker_of(cur - (unsigned)s.x0 + (unsigned)s.blocks - 1);
-            s.xa = s.x0;
-            s.xb = s.x1;
-        } else {
-            const int cuts = (int)((s.blocks + longest - 1) / longest);
-            unit = inside / (unsigned)cuts;
-            const int cut = (int)(inside - unit * (unsigned)cuts), piece = s.blocks / cuts, rest = s.blocks - piece * cuts;
-            s.x0 = piece * cut + min(cut, rest);
-            s.x1 = s.x0 + piece + (cut < rest);
-            s.w0 = (int)cur - cut;
-            s.w1 = s.w0 + cuts - 1;
+        const unsigned unit = inside / (unsigned)s.blocks;
+        s.x0 = (int)(inside - unit * (unsigned)s.blocks);
+        s.x1 = s.x0 + (int)min((unsigned)(s.blocks - s.x0), end - cur);
+        s.w0 = w_first >= 0 ? w_first : (int)worker_of(cur - (unsigned)s.x0);
+        s.w1 = w_first >= 0 ? w_last : (int)worker_of(cur - (unsigned)s.x0 + (unsigned)s.blocks - 1);
+        s.xa = s.x0;
+        s.xb = s.x1;
+        if (!by_warp) {
             const int each = (s.x1 - s.x0) / KA_WARPS, over = (s.x1 - s.x0) % KA_WARPS;
             s.xa = s.x0 + each * warp + min(warp, over);
             s.xb = s.xa + each + (warp < over);
@@ -605,8 +617,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
         }
         /* the stretch's next unit is on its way while this one's result is written and, where it is shared, put together */
         const Segment done = s;
-        const unsigned slot_at = cur;
-        cur += by_warp ? s.x1 - s.x0 : 1;
+        cur += (unsigned)(s.x1 - s.x0);
         const bool go_on = cur < end;
         if (go_on) {
             s = segment(cur);
@@ -630,7 +641,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
         };
         const bool whole = done.x0 == 0 && done.x1 == done.blocks;
         const int w0 = done.w0, w1 = done.w1;
-        const size_t slot = by_warp ? 2 * (size_t)(warp * gridDim.x + blockIdx.x) + (done.x0 == 0 ? 1 : 0) : (size_t)slot_at;
+        const size_t slot = 2 * (size_t)worker + (done.x0 == 0 ? 1 : 0);
         unsigned* arrived = parts.arrived + (size_t)row * cache.kv_heads + head;
         auto out_of = [&](int col) { return out + (size_t)(row + col / group) * q_stride + (size_t)(head * group + col % group) * 128; };
 
@@ -663,7 +674,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
                     for (int base = 0; base < columns; base += KA_PASS) {
                         float top[KA_PASS], sum[KA_PASS];
                         float4 acc[KA_PASS];
-                        ka_gather<COLS>(parts, 2, w0, w0, 1, w1, base, columns, lane, top, sum, acc);
+                        ka_gather<COLS>(parts, w0, w0, 1, w1, base, columns, lane, top, sum, acc);
 #pragma unroll
                         for (int k = 0; k < KA_PASS; k++)
                             if (base + k < columns) ka_store(out_of(base + k) + 4 * lane, acc[k], sum[k]);
@@ -730,7 +741,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
                     for (int base = 0; base < columns; base += KA_PASS) {
                         float top[KA_PASS], sum[KA_PASS];
                         float4 acc[KA_PASS];
-                        ka_gather<COLS>(parts, 1, -1, w0 + warp, KA_WARPS, w1, base, columns, lane, top, sum, acc);
+                        ka_gather<COLS>(parts, w0, w0 + warp, KA_WARPS, w1, base, columns, lane, top, sum, acc);
 #pragma unroll
                         for (int k = 0; k < KA_PASS; k++) {
                             if (base + k < COLS && lane == 0) {
