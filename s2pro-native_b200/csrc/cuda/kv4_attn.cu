@@ -32,8 +32,8 @@ constexpr int KA_PASS = 4;                                         /* columns me
 constexpr int KA_MERGE_BYTES = KA_WARPS * KA_PASS * 128 * 4;
 constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 8;          /* blocks that make a worker worth its while */
 /* (Row, head) columns of a kv head up to which an entry is this kernel's rather than that of the tensor cores: alone, and next to longer slices, where
- * most bring a token.  us here and there, 32 / 8 heads: 4, 16, 32, 64 rows of one sequence at 1100 positions 16.9, 18.2, 19.5, 42 and 16.4, 18.1,
- * 20.3, 24.6; at 8000 positions 19.9, 27.6, 52, 61 and 27.9, 29.3, 33.4, 41.8; 4, 8, 16 rows of 16 sequences at 4000 53, 57, 82 and 72, 73, 75. */
+ * most bring a token.  us here and there, 32 query and 8 kv heads: 4, 8, 16, 32 rows of one sequence of 1100 positions 17.4, 18.8, 18.6, 19.9 and 17.6, 17.8,
+ * 18.3, 19.2; of 8000 positions 20.4, 22.3, 28.1, 48.9 and 24.0, 25.0, 25.8, 27.7; 4, 8 rows of 16 sequences of 4000 41.5, 53.9 and 80, 81. */
 constexpr int KA_FEW = 64, KA_FEW_BESIDE = 32;
 /* How the work is cut (us, 32 query and 8 kv heads, one row a sequence).  Units each cut into equal parts, one to a CTA, its warps joined through shared memory,
  * wherever there are no more units than CTAs: 15 sequences of 1500 13.0, by warps below 20.6; up to KA_LONG blocks to a warp, where the warps' barriers cost more

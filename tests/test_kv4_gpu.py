@@ -204,6 +204,56 @@ def test_a_long_slice(mine, capi):
         check_attention(cache, b, [(0, 7000 - n, 0, n)], q[:n], out)
 
 
+LINES = {
+    "no more than a warp's worth each": [1, 3, 16, 2, 40],
+    "parts of CTAs": [700, 640, 650, 700, 690, 610, 500, 700, 100],
+    "one far longer than the others": [6000] + [90, 100, 1, 64] * 4,
+    "parts of warps": [500, 513, 480, 511, 512, 497] * 4 + [513, 1],
+    "stretches of warps": [2100, 300, 64, 1, 1700, 900, 17, 3000] * 3,
+    "more units than warps": [33, 70, 1, 16, 128, 64, 99, 130, 5, 48] * 16,
+}
+
+
+@pytest.mark.parametrize("name", LINES)
+@pytest.mark.parametrize("q_heads,kv_heads", [(32, 8), (16, 1)])
+def test_lines_of_single_tokens(mine, capi, name, q_heads, kv_heads):
+    """Batches of single tokens that are cut in each of the ways there are, three times with the same bits."""
+    lens = LINES[name]
+    n = len(lens)
+    cache = _kv4.Cache(mine, capi, sum((x + 63) // 64 for x in lens) + 1, kv_heads=kv_heads, q_heads=q_heads, max_seqs=n, stride=96, rows=n)
+    for i, x in enumerate(lens):
+        _kv4.fill(cache, i, x, seed=i)
+    b = cache.batch(range(n), [1] * n, [x - 1 for x in lens])
+    q = queries(n, q_heads)
+    outs = []
+    for _ in range(3):
+        out = torch.full_like(q, 7.0)
+        cache.attention(b, q, out)
+        outs.append(out)
+    check_attention(cache, b, [(i, x - 1, i, 1) for i, x in enumerate(lens)], q, outs[0])
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("lens,counts", [([7000] + [50] * 12, [32] + [40] * 12), ([300, 250, 333], [70, 64, 65]), ([64] * 3, [33] * 3), ([4000, 3900], [300, 290])])
+def test_few_slices_of_unequal_lengths(mine, capi, lens, counts):
+    """No more units than SMs, cut into parts of their own or, where one is far longer, along one line."""
+    n, total = len(lens), sum(counts)
+    cache = _kv4.Cache(mine, capi, sum((x + 63) // 64 for x in lens) + 1, kv_heads=8, q_heads=32, max_seqs=n, stride=110, rows=total)
+    for i, x in enumerate(lens):
+        _kv4.fill(cache, i, x, seed=i)
+    firsts = [x - c for x, c in zip(lens, counts)]
+    b = cache.batch(range(n), counts, firsts)
+    q = queries(total, 32)
+    outs = []
+    for _ in range(2):
+        out = torch.full_like(q, 7.0)
+        cache.attention(b, q, out)
+        outs.append(out)
+    check_attention(cache, b, [(i, p, sum(counts[:i]), c) for i, (p, c) in enumerate(zip(firsts, counts))], q, outs[0])
+    assert torch.equal(outs[0], outs[1])
+    cache.call("status", None)
+
+
 def test_as_many_sequences_as_a_batch_takes(mine, capi):
     n = 1024
     cache = _kv4.Cache(mine, capi, 1100, kv_heads=1, q_heads=2, max_seqs=n, stride=2, rows=n + 40)
