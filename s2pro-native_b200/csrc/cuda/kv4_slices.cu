@@ -21,7 +21,7 @@
  *
  * The pages of all units form one line, and each CTA takes an equal stretch of it, wherever that cuts units.  With no more units than CTAs
  * most CTAs would get the end of one unit and the start of the next: there every unit is cut into equal parts of its own, one to a CTA
- * (32 query and 8 kv heads, 512 rows behind 1500: 49 -> 41 us, 77 rows behind 100: 30 -> 24.5).  The parts of a
+ * (32 query and 8 kv heads, 512 rows behind 1500: 49 -> 41 us, 77 behind 1024: 30 -> 24.5).  The parts of a
  * unit are added, in order, by a second kernel over all SMs: in the last CTA to arrive that took 8 us for two parts of 128 KB and 20 for
  * five, with the other SMs idle.  Parts stay in 32 bits (f16 would take 1.5 us off the smallest calls).
  * A page takes a CTA 1.25 us; the tensor cores are busy 54% of that, the rest is the softmax's and the converters' instructions. */
@@ -35,7 +35,7 @@ constexpr int KS_Q_PITCH = 128 * 16 + 16, KS_Q_BYTES = 16 * KS_Q_PITCH;         
 constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
 constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + 2 * KS_RAW * KV4_HEAD_BYTES;
-constexpr int KS_LEAST = 3;  /* pages that make a CTA worth its while: 77 rows behind 100 with 2 and 3: 26.9 and 25.2 us; longer calls have more in any case */
+constexpr int KS_LEAST = 3;  /* pages that make a CTA worth its while: 77 rows behind 1024 with 2 and 3: 26.9 and 25.2 us; longer calls have more in any case */
 constexpr int KS_SECOND = 4; /* pages that a second unit costs a CTA (5 us: queries, a part to write, another's to read) */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
