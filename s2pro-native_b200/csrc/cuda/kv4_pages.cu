@@ -100,14 +100,29 @@ __device__ __forceinline__ int kv4_held(const Kv4Book& k, int seq) {
 
 __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_reserve(Kv4Book k, s2p_b200_kv4_batch b, int32_t* info) {
     __shared__ int sh[33], upto[S2P_B200_KV4_MAX_BATCH], first_of[S2P_B200_KV4_MAX_BATCH], seq_of[S2P_B200_KV4_MAX_BATCH];
+    constexpr int SLOTS = 2 * S2P_B200_KV4_MAX_BATCH;
+    __shared__ int named[SLOTS], first_named[SLOTS]; /* the sequences that stand in the batch, and where first */
+    const int e = threadIdx.x;
+    for (int i = e; i < SLOTS; i += KV4_SCAN_THREADS) {
+        named[i] = -1;
+        first_named[i] = S2P_B200_KV4_MAX_BATCH;
+    }
+    __syncthreads();
     grid_wait();
     grid_release();
-    const int e = threadIdx.x;
-    int seq = -1, held = 0, need = 0, fits = 0;
+    int seq = -1, held = 0, need = 0, fits = 0, slot = 0;
     long long after = 0;
     if (e < b.n) {
         seq = b.seqs[e];
         if ((unsigned)seq < (unsigned)k.max_seqs) {
+            slot = (int)((unsigned)seq * 2654435769u >> 16) % SLOTS; /* (2^32 over the golden ratio) */
+            for (int there; (there = atomicCAS(&named[slot], -1, seq)) != -1 && there != seq;) slot = (slot + 1) % SLOTS; /* at most half of them are taken */
+            atomicMin(&first_named[slot], e);
+        }
+    }
+    __syncthreads();
+    if (e < b.n) {
+        if ((unsigned)seq < (unsigned)k.max_seqs && first_named[slot] == e) {
             held = kv4_held(k, seq);
             after = (long long)held + max(0, min(b.row0[e + 1], b.rows) - max(b.row0[e], 0));
             fits = after <= (long long)k.stride * S2P_B200_KV4_PAGE;

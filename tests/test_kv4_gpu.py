@@ -649,6 +649,26 @@ def test_pool_runs_out_in_order(mine, capi):
     book.check(cache, book.fork([0, 1], [4, 5], [90, -1]))
 
 
+def test_a_sequence_that_stands_in_a_batch_twice(mine, capi):
+    """Reserve serves the first entry and refuses the others; no page is lost."""
+    n = 1024
+    cache = _kv4.Cache(mine, capi, 900, kv_heads=1, q_heads=1, max_seqs=5000, stride=4, rows=3 * n)
+    seqs = [i * 37 % 400 * 7 for i in range(n)]
+    b = cache.batch(seqs, [1 + i % 3 for i in range(n)])
+    cache.reserve(b)
+    torch.cuda.synchronize()
+    seen, want = set(), []
+    for s in seqs:
+        want.append(-1 if s in seen else 0)
+        seen.add(s)
+    assert b.pos0.cpu().tolist() == want
+    assert cache.info.cpu().tolist() == [900 - len(seen), n - len(seen)]
+    assert sorted(cache.table[cache.table >= 0].cpu().tolist()) == list(range(len(seen)))
+    cache.reserve(cache.batch([3, 4, 3, -1, 5000, 4], [1, 0, 70, 1, 1, 0]))
+    torch.cuda.synchronize()
+    assert cache.info.cpu().tolist()[1] == 4
+
+
 def test_empty_and_unusual_calls(mine, capi):
     cache = marked(mine, capi, 5, layers=1, kv_heads=1, q_heads=1, max_seqs=3, stride=2)
     book = Book(cache)
