@@ -15,9 +15,9 @@ namespace s2p {
 
 constexpr int KV4_ROW_WARPS = 8, KV4_ROWS = 4, KV4_AHEAD = 3; /* warps and rows of a CTA; pairs of vectors whose loads a warp has under way */
 
-/* cosine and sine of pair i at position pos; per_pair = log2(base) / 64 */
-__device__ __forceinline__ float2 kv4_turn(int pos, int i, double per_pair) {
-    double turns = (double)pos * exp2(-(double)i * per_pair) * 0.15915494309189533577; /* angle / 2 pi */
+/* cosine and sine of a pair at position pos; per_position: the turns that it makes from one to the next */
+__device__ __forceinline__ float2 kv4_turn(int pos, double per_position) {
+    double turns = (double)pos * per_position;
     turns -= rint(turns);
     float s, c;
     sincospif(2.0f * (float)turns, &s, &c);
@@ -37,17 +37,19 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4View& cache, const Kv4Row
 /* A CTA has `rows` (up to KV4_ROWS) consecutive rows, whose places and angles it works out once, and its warps their pairs of head vectors in turn. */
 __global__ void __launch_bounds__(KV4_ROW_WARPS * 32, 4)
 k_kv4_append(Kv4View cache, Kv4Rows b, int rows, const __nv_bfloat16* qkv, const __nv_bfloat16* q_norm, const __nv_bfloat16* k_norm, float eps,
-             double per_pair, __nv_bfloat16* q) {
+             double per_pair /* log2(base) / 64 */, __nv_bfloat16* q) {
     __shared__ __align__(16) float2 turn[KV4_ROWS][64];
     __shared__ Kv4Place place[KV4_ROWS];
     const int row0 = blockIdx.x * rows, l = threadIdx.x & 15, second = (threadIdx.x >> 4) & 1;
     const unsigned half = 0xFFFFu << (16 * second);
     const int heads = cache.q_heads + 2 * cache.kv_heads, step = KV4_ROW_WARPS * gridDim.y, first = blockIdx.y * KV4_ROW_WARPS + (threadIdx.x >> 5);
+    static_assert(KV4_ROW_WARPS * 32 % 64 == 0, "a thread's angles are of one pair of channels");
+    const double per_position = exp2(-(double)(threadIdx.x & 63) * per_pair) * 0.15915494309189533577; /* 1 / 2 pi */
     grid_wait();
     grid_release();
     if (threadIdx.x < rows) place[threadIdx.x] = kv4_place(cache, b, row0 + threadIdx.x);
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * rows; i += KV4_ROW_WARPS * 32) turn[i >> 6][i & 63] = kv4_turn(max(place[i >> 6].pos, 0), i & 63, per_pair);
+    for (int i = threadIdx.x; i < 64 * rows; i += KV4_ROW_WARPS * 32) turn[i >> 6][i & 63] = kv4_turn(max(place[i >> 6].pos, 0), per_position);
     __syncthreads();
     for (int r = 0; r < rows; r++) {
         const int pos = place[r].pos, page = place[r].page;
@@ -119,11 +121,12 @@ k_kv4_append(Kv4View cache, Kv4Rows b, int rows, const __nv_bfloat16* qkv, const
     }
 }
 
-/* Rows to a CTA and CTAs to them: several rows where there are many, several CTAs where there are few. */
+/* Rows to a CTA and CTAs to them: as many rows as leave the CTAs one wave of four to an SM, up to four (2055 rows: 1, 2, 4, 8 to a CTA 31, 27.9, 26, 39 us;
+ * 1000 rows: 2 to a CTA 15, 4 in two CTAs 19.4), several CTAs where there are few. */
 struct Kv4RowGrid { dim3 grid; int rows; };
 static Kv4RowGrid kv4_row_grid(int rows, int vectors) {
     Kv4RowGrid g;
-    g.rows = rows >= 148 * KV4_ROWS ? KV4_ROWS : 1;
+    g.rows = rows <= 3 * 592 ? (rows + 591) / 592 : KV4_ROWS;
     const int x = (rows + g.rows - 1) / g.rows, most = ((vectors + 1) / 2 + KV4_ROW_WARPS - 1) / KV4_ROW_WARPS;
     const int want = (2 * 148 + x - 1) / x;
     g.grid = dim3((unsigned)x, (unsigned)(want < most ? want : most));

@@ -746,7 +746,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
 }
 
 /* The parts of shared units, in order of the CTAs that left them.  Block (w, y): 32 rows of the unit that CTA w began; a thread has one unit of eight
- * columns of a row, and eight parts' loads are under way at a time. */
+ * columns of a row, and four parts' loads are under way at a time (eight: the same). */
 constexpr int KS_JOIN_ROWS = 32, KS_JOIN_THREADS = 16 * KS_JOIN_ROWS, KS_JOIN_PARTS = 4;
 __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int q_heads, int group, __nv_bfloat16* out) {
     grid_wait();

@@ -165,7 +165,10 @@ def attention(cache, seq, first, q, layer=0):
     The kernel rounds a weight p to f16 (2^-11 of it) and p s to f16 (2^-11 again); the sum of weights is not rounded.  So a value's part
     s c p / sum is off by at most 2^-10 of it, the part m p / sum by 2^-11 (second order: 2^-20); scores and their
     exponentials are in 32 bits (|logit| < 64 here: 2^-24 * 64 * a few, below 2^-15 of a weight).  A weight or a product below f16's normal range is off by 2^-25 at most,
-    over 4 for the head room, and the largest weight is at least 1, so the sum is: 2^-25 (15 + |v|) for each position.  And the result is rounded to bf16: 2^-8 of it."""
+    over 4 for the head room, and the largest weight is at least 1, so the sum is: 2^-25 (15 + |v|) for each position.  And the result is rounded to bf16: 2^-8 of it.
+
+    For prompt slices it is a value s c + m that is rounded to f16 in place of p s, 2^-11 again.  Keys are, too, which moves a logit by 2^-11 sum |q k| / sqrt(128) at the
+    worst; the bound leaves no room for that (of 128 channels and many positions, of either sign, little is left), so it asks for more than the worst case."""
     rows, group = q.shape[0], cache.q_heads // cache.kv_heads
     k, v, mass, there = cache.values(seq, first + rows, layer)
     x = q.double().cpu().view(rows, cache.kv_heads, group, 128)
