@@ -612,7 +612,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 ok = ok && (turn == 0 || ks_wait_warp(&bars.k_free[stage], (turn - 1) & 1, status));
                 unsigned char* to = sk + stage * KS_K_BYTES;
                 if (ok) {
-#pragma unroll
+#pragma unroll 1
                     for (int j = 0; j < 2; j++) { /* this thread's units are in blocks p >> 6 and 2 + (p >> 6) */
                         const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
                         const uint4 kc = *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16), kp = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16));
