@@ -42,7 +42,7 @@ static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 =
 struct KsBars {
     uint64_t k_full[KS_STAGES], k_free[KS_STAGES], v_full[KS_STAGES], v_free[KS_STAGES];
     uint64_t s_full[2][2], p_full[2][2]; /* [row tile][place] */
-    uint64_t o_done[2], q_full, q_free, unit_done, all_done[2];
+    uint64_t o_done[2], q_full, q_free, unit_done[2], all_done[2];
 };
 
 struct KsLine { /* in shared memory: the chunks (units of one kv head each) of all entries */
@@ -204,11 +204,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 mbar_init(&bars.p_full[i][j], 4);
             }
             mbar_init(&bars.o_done[i], 1);
+            mbar_init(&bars.unit_done[i], 1);
             mbar_init(&bars.all_done[i], 1);
         }
         mbar_init(&bars.q_full, 8);
         mbar_init(&bars.q_free, 2);
-        mbar_init(&bars.unit_done, 2);
         mbar_init_fence();
     }
     grid_wait();
@@ -450,7 +450,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         const int x = warp >> 2, r = tid & 127; /* row tile, row */
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_o = tmem + (uint32_t)(x * 128) + lanes, t_s = tmem + 256u + (uint32_t)(x * 128) + lanes;
-        unsigned n_s = 0, segments = 0; /* pages of this row tile so far */
+        unsigned n_s = 0, segments = 0, units = 0; /* pages of this row tile so far; units; those in which it has rows */
         bool ok = true, begun = false;
         int chunk = chunk_at;
         unsigned it = 0; /* pages of the CTA so far */
@@ -526,8 +526,10 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     if (lane == 0) mbar_arrive(&bars.p_full[x][place]);
                 }
             it += (unsigned)(s.t1 - s.t0);
-            if (ok) {
-                ok = ks_wait_warp(&bars.unit_done, segments & 1, status);
+            /* The unit's last product of this row tile.  A barrier for each tile, of the units in which it has rows: an issuer without any is done with its unit, and
+             * with the next, before the other one is.  (Its next phase needs this tile's weights, so it is never two ahead.) */
+            if (ok && active) {
+                ok = ks_wait_warp(&bars.unit_done[x], units++ & 1, status);
                 ks_after_sync();
             }
             segments++;
@@ -724,7 +726,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     stage = next;
                     turn = next_turn;
                 }
-                if (ok) ks_commit(&bars.unit_done);
+                if (ok && active) ks_commit(&bars.unit_done[x]);
                 cur += (unsigned)(s.t1 - s.t0);
             }
             /* TMEM must not be freed under products in flight: they complete by themselves, and this waits for them with a limit of its own */

@@ -254,6 +254,29 @@ def test_few_slices_of_unequal_lengths(mine, capi, lens, counts):
     cache.call("status", None)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads", [(48, 3), (32, 8)])
+def test_many_slices_of_few_rows(mine, capi, q_heads, kv_heads):
+    """Units with rows in one of their two tiles, several to a CTA: a result is not read before its last product, whatever the other tile does meanwhile."""
+    n, group = 200, q_heads // kv_heads
+    counts = [9 * 4 // group + i % 7 for i in range(n)]
+    lens = [c + 60 + 7 * (i % 13) for i, c in enumerate(counts)]
+    total = sum(counts)
+    cache = _kv4.Cache(mine, capi, sum((x + 63) // 64 for x in lens) + 1, kv_heads=kv_heads, q_heads=q_heads, max_seqs=n, stride=4, rows=total)
+    for i, x in enumerate(lens):
+        _kv4.fill(cache, i, x, seed=i)
+    firsts = [x - c for x, c in zip(lens, counts)]
+    b = cache.batch(range(n), counts, firsts, max_rows=1000)
+    q = queries(total, q_heads)
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    check_attention(cache, b, [(i, firsts[i], sum(counts[:i]), counts[i]) for i in range(0, n, 9)], q, out)
+    for _ in range(200):
+        again = torch.full_like(q, 7.0)
+        cache.attention(b, q, again)
+        assert torch.equal(again, out)
+    cache.call("status", None)
+
+
 def test_as_many_sequences_as_a_batch_takes(mine, capi):
     n = 1024
     cache = _kv4.Cache(mine, capi, 1100, kv_heads=1, q_heads=2, max_seqs=n, stride=2, rows=n + 40)
