@@ -440,6 +440,27 @@ def test_append(mine, capi, q_heads, kv_heads, first, rows):
         assert torch.equal(cache.pages[unwritten], before[unwritten])
 
 
+@pytest.mark.parametrize("rows", [296, 592, 593, 1185, 1777, 2371])
+def test_append_and_read_many_rows(mine, capi, rows):
+    """From one row to four of a CTA, the last of them partly padding."""
+    cache = _kv4.Cache(mine, capi, 40, kv_heads=1, q_heads=3, stride=40, rows=rows + 3)
+    counts = [rows - 100, 100]
+    b = cache.batch([1, 3], counts, rows=rows + 3)
+    cache.reserve(b)
+    qkv = queries(rows + 3, 5)
+    q = torch.full((rows + 3, 3 * 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    cache.append(b, qkv, q)
+    check_append(cache, b, [(1, 0, 0, counts[0]), (3, 0, counts[0], 100)], qkv, q, None, None, 1e-6, 1e6)
+    assert bool((q[rows:] == 7).all())
+    got = [torch.full((rows + 3, 128), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    cache.call("read", C.byref(b.c), 0, got[0].data_ptr(), got[1].data_ptr(), None)
+    torch.cuda.synchronize()
+    for seq, r0, n in ((1, 0, counts[0]), (3, counts[0], 100)):
+        for out, held in zip(got, cache.values(seq, n)[:2]):
+            assert torch.equal(out[r0:r0 + n].cpu(), held[0].bfloat16())
+    assert all(bool((out[rows:] == 7).all()) for out in got)
+
+
 def test_append_far_positions(mine, capi):
     """Positions near the end of the longest sequence of this repository: the angle of the fastest pair is 32767 radians."""
     cache = _kv4.Cache(mine, capi, 20, kv_heads=2, q_heads=8, stride=512)
