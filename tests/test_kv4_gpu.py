@@ -856,6 +856,45 @@ def test_a_captured_tick_replays_as_the_sequences_grow(mine, capi):
     assert torch.equal(cache.table, again.table) and cache.lens.cpu().tolist() == [162, 101, 0, 230]
 
 
+def test_captured_mixed_batches_with_one_workspace(mine, capi):
+    """Two graphs on one workspace, of slices and of tokens; what the batches hold changes between replays."""
+    hq, hk, n, rows = 8, 2, 6, 260
+    cache = _kv4.Cache(mine, capi, 80, kv_heads=hk, q_heads=hq, max_seqs=n, stride=16, rows=rows)
+    other = _kv4.Cache(mine, capi, 80, kv_heads=hk, q_heads=hq, max_seqs=n, stride=16, rows=rows)
+    lens = [700, 64, 300, 129, 500, 260]
+    for i, x in enumerate(lens):
+        _kv4.fill(cache, i, x, seed=i)
+    other.pages.copy_(cache.pages)
+    other.table.copy_(cache.table)
+    q = queries(rows, hq)
+    slices, tokens = cache.batch(range(n), [0] * n, [0] * n, rows=rows, max_rows=rows), cache.batch(range(n), [1] * n, [0] * n)
+    out, out1 = torch.zeros_like(q), torch.zeros_like(q[:n])
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graphs = []
+    for b, to in ((slices, out), (tokens, out1)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            cache.attention(b, q, to, stream=C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        graphs.append(g)
+    for counts in ([1, 64, 1, 1, 100, 1], [200, 1, 33, 2, 1, 0], [1] * 6, [0, 0, 0, 0, 0, 260], [5, 40, 60, 7, 50, 40]):
+        row0 = [0]
+        for c in counts:
+            row0.append(row0[-1] + c)
+        slices.row0.copy_(torch.tensor(row0, dtype=torch.int32))
+        slices.pos0.copy_(torch.tensor([x - c for x, c in zip(lens, counts)], dtype=torch.int32))
+        tokens.pos0.copy_(torch.tensor([x - 1 - counts[0] % 7 for x in lens], dtype=torch.int32))
+        for g, b, to in ((graphs[0], slices, out), (graphs[1], tokens, out1)) * 2:
+            to.fill_(7.0)
+            g.replay()
+            want = torch.full_like(to, 7.0)
+            other.attention(b, q, want)
+            torch.cuda.synchronize()
+            assert torch.equal(to, want)
+        check_attention(cache, slices, [(i, lens[i] - c, row0[i], c) for i, c in enumerate(counts) if c], q, out)
+    cache.call("status", None)
+
+
 def test_a_wait_that_gives_up_is_told_and_leaves_nothing_behind(testlib, capi):
     """The deadline of the slices' bounded waits lowered until one runs out: the call ends, the status says so once, and with the deadline
     restored the next call is right."""
