@@ -168,7 +168,7 @@ def attention(cache, seq, first, q, layer=0):
     over 4 for the head room, and the largest weight is at least 1, so the sum is: 2^-25 (15 + |v|) for each position.  And the result is rounded to bf16: 2^-8 of it.
 
     For prompt slices it is a value s c + m that is rounded to f16 in place of p s, 2^-11 again.  Keys are, too, which moves a logit by 2^-11 sum |q k| / sqrt(128) at the
-    worst; the bound leaves no room for that (of 128 channels and many positions, of either sign, little is left), so it asks for more than the worst case."""
+    worst; the bound leaves no room for that (of 128 channels and many positions, of either sign, little is left): it is narrower than the worst case."""
     rows, group = q.shape[0], cache.q_heads // cache.kv_heads
     k, v, mass, there = cache.values(seq, first + rows, layer)
     x = q.double().cpu().view(rows, cache.kv_heads, group, 128)
