@@ -38,10 +38,12 @@ constexpr int KA_FEW = 64, KA_FEW_BESIDE = 32;
 /* How the work is cut (us, 32 query and 8 kv heads, one row a sequence).  Units each cut into equal parts, one to a CTA, its warps joined through shared memory,
  * wherever there are no more units than CTAs: 15 sequences of 1500 13.0, by warps below 20.6; up to KA_LONG blocks to a warp, where the warps' barriers cost more
  * than the partials that they save (9 of 8000 28.2 and 27.5, 12 of 4000 24.0 and 22.8), and where no part has KA_SECOND blocks more than an equal share (one
- * sequence of 2000 among 15 of 1000, 67 more: 14.6 and 16.4; of 3000, 130 more: 18.2 and 17.8).  Otherwise a warp is a worker by itself and leaves a partial.
+ * sequence of 2000 among 15 of 1000, 67 more: 14.6 and 16.4; of 3000, 130 more: 18.2 and 17.8).  Units of up to KA_WHOLE blocks are not cut even so, since putting
+ * parts together takes longer than more blocks do (one sequence of 512 whole 7.8, cut 9.0; 8 of 1000 11.0 and 12.0, of 1250 11.7 and 12.0; one of 1000 9.9 and 9.6, of
+ * 1100 10.9 and 9.7).  Otherwise a warp is a worker by itself and leaves a partial.
  * Equal parts of each unit again (64 of 512: 18.0, 24 of 2500: 23.5), unless a part has KA_SECOND_WARP blocks more than an equal stretch of the line of all units'
  * blocks, in which many warps end one unit and begin the next (64 of 512 20.5, 24 of 2500 26.2; but 32 of 8192, 18 more: 58.5, in parts 66). */
-constexpr int KA_SECOND = 120, KA_SECOND_WARP = 8, KA_LONG = 20;
+constexpr int KA_SECOND = 120, KA_SECOND_WARP = 8, KA_LONG = 20, KA_WHOLE = 64;
 
 struct KaBatch { /* in shared memory, [n (+ 1)] */
     unsigned* upto;  /* blocks of all units before entry e */
@@ -468,7 +470,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
         /* parts of at most this many blocks are no more than there are workers; the longest of those parts */
         auto cut_for = [&](unsigned workers, unsigned least) { return max(least, (total + workers - units - 1) / (workers - units)); };
         auto part_of = [&](unsigned cut) { return cut ? (most + (most + cut - 1) / cut - 1) / max(1u, (most + cut - 1) / cut) : 0u; };
-        unsigned cut = units < grid && total < warps * KA_LONG ? cut_for(grid, KA_LEAST_CTA) : 0;
+        unsigned cut = units < grid && total < warps * KA_LONG ? most <= KA_WHOLE ? max(most, 1u) : cut_for(grid, KA_LEAST_CTA) : 0;
         bool by_warp = !cut || part_of(cut) > total / grid + KA_SECOND;
         if (by_warp) {
             cut = units < warps ? cut_for(warps, KA_LEAST_WARP) : 0;
