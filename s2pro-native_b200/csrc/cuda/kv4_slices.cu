@@ -37,6 +37,7 @@ constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
 constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + 2 * KS_RAW * KV4_HEAD_BYTES;
 constexpr int KS_LEAST = 3;  /* pages that make a CTA worth its while: 77 rows behind 1024 with 2 and 3: 26.9 and 25.2 us; longer calls have more in any case */
+constexpr int KS_UNIT = 6;   /* pages that a unit costs a CTA besides its own: a prompt's first units have one page, two, ... */
 constexpr int KS_SECOND = 4; /* pages that a second unit costs a CTA (5 us: queries, a part to write, another's to read) */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
@@ -275,7 +276,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
             const int c = c0 + lane;
             const int t = c < (int)chunks ? tiles_of(entry_of(c), c) : 0;
             most = max(most, t);
-            const unsigned at = before((unsigned)t * (unsigned)cache.kv_heads, total);
+            const unsigned at = before(t ? (unsigned)(KS_UNIT + t) * (unsigned)cache.kv_heads : 0u, total);
             if (c <= (int)chunks) line.upto[c] = at;
         }
         most = (int)__reduce_max_sync(S2P_FULL_MASK, (unsigned)most);
@@ -283,11 +284,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         /* As many units as CTAs or fewer: each is cut into parts of at most `longest` pages, the shortest for which there is a CTA to each part; unless a
          * CTA's equal share of the line is shorter by more than a second unit costs it (its queries, its part, and the other's reading of it). */
         const unsigned heads = (unsigned)cache.kv_heads;
-        unsigned workers = min(gridDim.x, (total + KS_LEAST - 1) / KS_LEAST), longest = 0;
+        unsigned workers = min(gridDim.x, max(total / (KS_UNIT + KS_LEAST), min(total, 1u))), longest = 0; /* (a stretch longer than what a unit costs has pages) */
         if (chunks * heads <= gridDim.x && chunks) {
             auto parts_at = [&](unsigned l) {
                 unsigned n = 0;
-                for (int c = lane; c < (int)chunks; c += 32) n += ((line.upto[c + 1] - line.upto[c]) / heads + l - 1) / l;
+                for (int c = lane; c < (int)chunks; c += 32) n += ((line.upto[c + 1] - line.upto[c]) / heads - KS_UNIT + l - 1) / l;
                 return __reduce_add_sync(S2P_FULL_MASK, n) * heads;
             };
             unsigned lo = KS_LEAST, hi = max((unsigned)most, (unsigned)KS_LEAST);
@@ -296,18 +297,18 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 if (parts_at(mid) <= gridDim.x) hi = mid;
                 else lo = mid + 1;
             }
-            if (lo <= total / gridDim.x + KS_SECOND) {
+            if (lo <= total / workers + KS_SECOND) {
                 longest = lo;
                 workers = 0;
                 if (lane == 0) sh_line.begin = sh_line.end = 0;
                 __syncwarp();
                 for (int c0 = 0; c0 < (int)chunks; c0 += 32) {
                     const int c = c0 + lane;
-                    const unsigned t = c < (int)chunks ? (line.upto[c + 1] - line.upto[c]) / heads : 0u, cuts = (t + longest - 1) / longest;
+                    const unsigned t = c < (int)chunks ? (line.upto[c + 1] - line.upto[c]) / heads - KS_UNIT : 0u, cuts = (t + longest - 1) / longest;
                     const unsigned at = before(cuts * heads, workers);
                     if (blockIdx.x >= at && blockIdx.x - at < cuts * heads) {
                         const unsigned head = (blockIdx.x - at) / cuts, cut = blockIdx.x - at - head * cuts, each = t / cuts, over = t - each * cuts;
-                        sh_line.begin = line.upto[c] + head * t + each * cut + min(cut, over);
+                        sh_line.begin = line.upto[c] + head * (KS_UNIT + t) + KS_UNIT + each * cut + min(cut, over);
                         sh_line.end = sh_line.begin + each + (cut < over);
                         sh_line.last = blockIdx.x - cut + cuts - 1;
                     }
@@ -327,10 +328,12 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     ks_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh_tmem);
     const unsigned chunks = (unsigned)line.first[b.n], worker = blockIdx.x;
-    const unsigned begin = sh_line.begin, end = sh_line.end;
+    const unsigned begin = sh_line.begin;
+    unsigned end = sh_line.end;
 
     struct Segment {
         int e, head, row0, n_rows, seq, p0, seen, t0, t1, tiles, r0; /* pages t0 .. t1 - 1 of `tiles` */
+        unsigned next;                                              /* where the stretch's next unit begins */
     };
     int chunk_at = 0;
     if (begin < end) {
@@ -341,9 +344,18 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         }
         chunk_at = lo;
     }
+    if (begin < end) { /* a stretch may end before the first page of its last unit */
+        int lo = chunk_at, hi = (int)chunks;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (line.upto[mid] < end) lo = mid; else hi = mid;
+        }
+        const unsigned inside = end - line.upto[lo], unit = (unsigned)(KS_UNIT + tiles_of(entry_of(lo), lo)), at = inside % unit;
+        if (at && at <= (unsigned)KS_UNIT) end -= at;
+    }
     auto last_of = [&](const Segment& s, unsigned cur) { /* the last CTA of the unit that this one begins */
         if (sh_line.last) return sh_line.last;
-        const unsigned x = cur + (unsigned)s.tiles - 1, longer = (sh_line.share + 1) * sh_line.more;
+        const unsigned x = cur + (unsigned)s.tiles - 1 /* from its first page */, longer = (sh_line.share + 1) * sh_line.more;
         return x < longer ? x / (sh_line.share + 1) : sh_line.more + (x - longer) / sh_line.share;
     };
     auto segment = [&](unsigned cur, int& chunk) {
@@ -352,9 +364,12 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         s.e = entry_of(chunk);
         s.tiles = tiles_of(s.e, chunk);
         const unsigned inside = cur - line.upto[chunk];
-        s.head = (int)(inside / (unsigned)s.tiles);
-        s.t0 = (int)(inside - (unsigned)s.head * (unsigned)s.tiles);
-        s.t1 = s.t0 + (int)min((unsigned)(s.tiles - s.t0), end - cur);
+        const unsigned long_ = (unsigned)(KS_UNIT + s.tiles);
+        s.head = (int)(inside / long_);
+        const unsigned at = inside - (unsigned)s.head * long_;
+        s.next = cur + min(long_ - at, end - cur);
+        s.t0 = max((int)at - KS_UNIT, 0);
+        s.t1 = (int)(at + (s.next - cur)) - KS_UNIT;
         s.r0 = (chunk - line.first[s.e]) * unit_rows;
         s.n_rows = min(unit_rows, rows_of(s.e) - s.r0);
         s.row0 = line.start[s.e] + s.r0;
@@ -375,7 +390,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     if (f_i == f.t1 - f.t0) {
                         if (f_cur == end) break;
                         f = segment(f_cur, f_chunk);
-                        f_cur += (unsigned)(f.t1 - f.t0);
+                        f_cur = f.next;
                         f_i = 0;
                     }
                     if ((f_i & 31) == 0) {
@@ -577,9 +592,9 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     parts.sum[slot * KS_SOFTMAX + tid] = sum;
                 }
             }
-            if (tid == 0 && s.t0 == 0 && !whole) parts.unit[worker] = make_int4(s.row0, s.n_rows, s.head, (int)last_of(s, cur));
+            if (tid == 0 && s.t0 == 0 && !whole) parts.unit[worker] = make_int4(s.row0, s.n_rows, s.head, (int)last_of(s, s.next - (unsigned)s.t1));
             begun |= s.t0 == 0 && !whole;
-            cur += (unsigned)(s.t1 - s.t0);
+            cur = s.next;
         }
         if (tid == 0 && !begun) parts.unit[blockIdx.x] = make_int4(0, 0, 0, 0);
     } else if (warp >= 8 && warp < 16) {
@@ -660,7 +675,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 if (!have_q) next_queries();
             }
             if (!have_q) next_queries();
-            cur += (unsigned)(s.t1 - s.t0);
+            cur = s.next;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp >= 16) {
@@ -728,7 +743,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     turn = next_turn;
                 }
                 if (ok && active) ks_commit(&bars.unit_done[x]);
-                cur += (unsigned)(s.t1 - s.t0);
+                cur = s.next;
             }
             /* TMEM must not be freed under products in flight: they complete by themselves, and this waits for them with a limit of its own */
             ks_commit(&bars.all_done[x]);
