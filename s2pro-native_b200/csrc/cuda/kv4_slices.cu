@@ -19,7 +19,7 @@
  * core-matrix layout (8 rows x 16 bytes); a unit plane has 32 or 16 bytes more than its positions take, so that the converting lanes'
  * stores fall on different banks.
  *
- * The pages of all units form one line, and each CTA takes an equal stretch of it, wherever that cuts units.  With no more units than CTAs
+ * The pages of all units, and what each costs besides, form one line, and each CTA takes an equal stretch of it, wherever that cuts units.  With no more units than CTAs
  * most CTAs would get the end of one unit and the start of the next: there every unit is cut into equal parts of its own, one to a CTA
  * (32 query and 8 kv heads, 512 rows behind 1500: 49 -> 41 us, 77 behind 1024: 30 -> 24.5).  The parts of a
  * unit are added, in order, by a second kernel over all SMs: in the last CTA to arrive that took 8 us for two parts of 128 KB and 20 for
@@ -37,7 +37,9 @@ constexpr int KS_K_PITCH = KS_TILE * 16 + 32, KS_V_PITCH = KS_TILE * 16 + 16;
 constexpr int KS_K_BYTES = 16 * KS_K_PITCH, KS_V_BYTES = 16 * KS_V_PITCH;
 constexpr int KS_OPERANDS = 2 * KS_Q_BYTES + KS_STAGES * (KS_K_BYTES + KS_V_BYTES) + 2 * KS_RAW * KV4_HEAD_BYTES;
 constexpr int KS_LEAST = 3;  /* pages that make a CTA worth its while: 77 rows behind 1024 with 2 and 3: 26.9 and 25.2 us; longer calls have more in any case */
-constexpr int KS_UNIT = 6;   /* pages that a unit costs a CTA besides its own: a prompt's first units have one page, two, ... */
+/* Pages that a unit costs a CTA besides its own: a prompt's first units have one page, two, ..., and without this a few CTAs get them all.  Prompts of 1000, 2000, 4000 from
+ * their first position with 0, 4, 6, 9: 88, 39, 39, 40 us; 190, 88, 83, 83; 431, 236, 200, 202. */
+constexpr int KS_UNIT = 6;
 constexpr int KS_SECOND = 4; /* pages that a second unit costs a CTA (5 us: queries, a part to write, another's to read) */
 static_assert(KS_OPERANDS % 16 == 0 && KS_K_BYTES % 16 == 0 && KS_V_BYTES % 16 == 0, "descriptors count 16 bytes");
 
@@ -282,7 +284,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
         most = (int)__reduce_max_sync(S2P_FULL_MASK, (unsigned)most);
         __syncwarp();
         /* As many units as CTAs or fewer: each is cut into parts of at most `longest` pages, the shortest for which there is a CTA to each part; unless a
-         * CTA's equal share of the line is shorter by more than a second unit costs it (its queries, its part, and the other's reading of it). */
+         * CTA's equal share of the line is shorter by more than a second unit costs it (a part to write, another's to read). */
         const unsigned heads = (unsigned)cache.kv_heads;
         unsigned workers = min(gridDim.x, max(total / (KS_UNIT + KS_LEAST), min(total, 1u))), longest = 0; /* (a stretch longer than what a unit costs has pages) */
         if (chunks * heads <= gridDim.x && chunks) {
