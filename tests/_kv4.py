@@ -180,3 +180,63 @@ def attention(cache, seq, first, q, layer=0):
     out = torch.einsum("rhgt,htd->rhgd", p, v)
     bound = torch.einsum("rhgt,htd->rhgd", p, mass) * (2 ** -10 + 2 ** -14) + (first + rows) * 2 ** -25 * (15 + v.abs().max())
     return out.reshape(rows, -1), bound.reshape(rows, -1) + out.abs().reshape(rows, -1) * 2 ** -8
+
+
+def store(cache, seq, keys, values, layer=0):
+    """Gives a sequence keys and values [kv_heads, length, 128] in free pages of a random order; positions behind the length keep what was there."""
+    heads, length, _ = keys.shape
+    n, dev = -(-length // PAGE), cache.pages.device
+    free = (cache.refs == 0).nonzero().flatten()
+    order = free[torch.randperm(len(free), generator=torch.Generator().manual_seed(length)).to(dev)[:n]]
+    cache.refs[order], cache.table[seq, :n], cache.lens[seq] = 1, order.int(), length
+    pos = torch.arange(length, device=dev)
+    page, block, place = order[pos // PAGE], pos % PAGE // 16, pos % 16
+    flat, half = cache.pages[:, layer].view(-1), cache.pages[:, layer].view(-1).view(torch.float16)
+    assert flat.data_ptr() == cache.pages.data_ptr()  # (caches of one layer)
+    for which, x in ((0, keys), (1, values)):
+        byte, _, at_s, at_m = (t.to(dev)[place] for t in places(which))
+        codes, s, m = quantise(x.to(dev).float())
+        for h in range(heads):
+            base = (((page * heads + h) * 4 + block) * BLOCK)[:, None]
+            flat[base + byte[:, 0::2]] = codes[h, :, 0::2] | codes[h, :, 1::2] << 4
+            half[(base + at_s) // 2], half[(base + at_m) // 2] = s[h], m[h]
+
+
+def attention_close(cache, seq, first, q, lift=12, layer=0):
+    """The result in 64 bits, and how far roundings that are independent of one another carry it: for sums of many positions this is far narrower than
+    the sum of worst cases in `attention`, and a part or a page that is left out shows.
+
+    With weights p_t (sum 1), |delta| <= 1 independent, a kernel returns sum_t p_t v_t + sum_t a_t delta_t, rounded to bf16 (2^-8 of it), where a_t collects
+      2^-11 p_t |v_t|             the weight in f16,
+      2^-11 p_t (s c + |m|)       the product p s, or the value s c + m, in f16,
+      2^-11 p_t |v_t - out| k_t   the keys in f16 for slices, k_t^2 = sum over channels of (q k)^2 / 128, by the softmax's derivative,
+      2^-15 p_t |v_t - out|       logits below 64 in 32 bits and their exponentials.
+    Hoeffding: |sum a delta| > 8 sqrt(sum a^2) has a probability below 2 e^-32.  Below f16's normal range a rounding is off by 2^-25: of a weight against the
+    largest (1 in slices, 2^lift for tokens, where values reach 2^(13 - lift) fifteenths): 2^-25 |v| or 2^-25 2^-lift 15 max(1, s) a position, in the same way."""
+    rows, heads, group, length = q.shape[0], cache.kv_heads, cache.q_heads // cache.kv_heads, first + q.shape[0]
+    n = -(-length // PAGE)
+    dev = cache.pages.device
+    entries = cache.table[seq, :n].long()
+    there = ((entries >= 0) & (entries < cache.n_pages)).repeat_interleave(PAGE)[:length]
+    blocks = cache.pages[entries.clamp(0, cache.n_pages - 1), layer]
+    half = blocks.view(torch.float16)
+    held = []
+    for which in (0, 1):
+        byte, shift, s, m = (t.to(dev) for t in places(which))
+        parts = [((blocks[..., byte] >> shift.to(torch.uint8)) & 15).double(), half[..., s // 2].double(), half[..., m // 2].double()]
+        parts = [t.permute(1, 0, 2, 3, 4).reshape(heads, n * PAGE, 128)[:, :length] for t in parts]
+        held += [torch.where(there[None, :, None], t, 0.0) for t in (parts[1] * parts[0] + parts[2], parts[1] * parts[0] + parts[2].abs(), parts[1])]
+    k, _, _, v, mass, s = held
+    x = q.double().view(rows, heads, group, 128)
+    z = torch.einsum("rhgd,htd->rhgt", x, k) / 128 ** 0.5
+    kk = torch.einsum("rhgd,htd->rhgt", x.square(), k.square()) / 128
+    seen = (torch.arange(length, device=dev) <= first + torch.arange(rows, device=dev)[:, None]) & there
+    p = torch.softmax(z.masked_fill(~seen[:, None, None], -torch.inf), -1)
+    out = torch.einsum("rhgt,htd->rhgd", p, v)
+    p2 = p.square()
+    near = p2 * (kk * 2.0 ** -22 + 2.0 ** -30)
+    spread = (torch.einsum("rhgt,htd->rhgd", near, v.square()) - 2 * out * torch.einsum("rhgt,htd->rhgd", near, v) + out.square() * near.sum(-1, keepdim=True)).clamp_min(0)
+    square = 2.0 ** -22 * torch.einsum("rhgt,htd->rhgd", p2, v.square() + mass.square()) + spread
+    small = p.amax(-1, keepdim=True) * (2.0 ** -25 * max(float(v.abs().max()), 15 * 2.0 ** -lift * max(1.0, float(s.max()))) * length ** 0.5)
+    bound = 8 * (square.sqrt() + small) * (1 + 2 ** -6) + out.abs() * 2 ** -8
+    return out.reshape(rows, -1), bound.reshape(rows, -1)
