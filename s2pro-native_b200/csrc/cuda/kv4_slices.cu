@@ -438,9 +438,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
 #pragma unroll
                 for (int off = 1; off < 16; off <<= 1) big = __vmaxu2(big, __shfl_xor_sync(S2P_FULL_MASK, big, off));
                 const int largest = (int)max(big & 0xFFFFu, big >> 16), e = largest ? min(136 - (largest >> 7), 120) : 0; /* 2^9 <= it times 2^e < 2^10 */
-                /* A query with an infinity or a NaN becomes NaN in all channels, and so do its scores: an infinity alone would make them infinite by the keys' signs, and a
-                 * row of nothing but -infinity looks like one that sees nothing. */
-                const float up = largest < 0x7F80 ? __uint_as_float((uint32_t)(127 + e) << 23) : __uint_as_float(0x7FFFFFFFu);
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                 if (r < KS_ROWS) {
                     if (u == 0) /* 2 log2(e) / sqrt(128) 2^-e */
                         sh_factor[unit & 3][tile * KS_ROWS + r] = __uint_as_float((uint32_t)(127 - e) << 23) * (2.0f * 1.4426950408889634f * 0.08838834764831845f);
@@ -540,6 +538,9 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     if (!ok) break;
                     const float2 both = ks_add2(s2[0], s2[1]);
                     sum += both.x + both.y;
+                    /* A query with an infinity makes scores infinite by the keys' signs, or NaN.  Where all that a row sees are -infinity it would look like one that sees
+                     * nothing, and that is zeros: */
+                    if (left > 0 && top == -INFINITY) sum = __uint_as_float(0x7FFFFFFFu);
                     ks_st_wait();
                     ks_before_sync();
                     __syncwarp();
