@@ -153,10 +153,15 @@ __device__ __forceinline__ uint32_t ks_half2(float lo, float hi) {
 }
 __device__ __forceinline__ __half2 ks_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t ks_u(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-/* Keys and values are held at half their size, so that the largest that the cache can stand for (65536) is an f16; scores and results are doubled
- * where they are scaled anyway. */
-__device__ __forceinline__ uint32_t ks_halve(uint32_t w) { return ks_u(__hmul2(ks_h2(w), ks_h2(0x38003800u))); }
-__device__ __forceinline__ uint4 ks_halve(const uint4& w) { return make_uint4(ks_halve(w.x), ks_halve(w.y), ks_halve(w.z), ks_halve(w.w)); }
+/* A group's largest code may stand for more than the 65504 that its largest value was kept at, by the roundings of m (16) and s (fifteen times 4): up to 65580, and from 65520
+ * on that is no f16.  m alone does not do it: with s < 32 the code would be 14.  True where one of the four s in x, y (z, w: m) is 32 or more; those operands are kept at
+ * 65504 by a second pass over them.  (Operands at half their size need no such pass, but s, m and s c + m below 2^-13 lose their last bit: scores of keys of 1e-5 were 6% off.) */
+__device__ __forceinline__ bool ks_wide(const uint4& w) { return (((w.x + 0x30003000u) | (w.y + 0x30003000u)) & 0x80008000u) != 0; }
+__device__ __forceinline__ uint32_t ks_keep(uint32_t w) { return ks_u(__hmin2(ks_h2(w), ks_h2(0x7BFF7BFFu))); }
+__device__ __forceinline__ void ks_keep(unsigned char* at) {
+    uint4* to = reinterpret_cast<uint4*>(at);
+    *to = make_uint4(ks_keep(to->x), ks_keep(to->y), ks_keep(to->z), ks_keep(to->w));
+}
 /* eight codes of a word as s c + m: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7 (those of a byte's upper half come as 16 c) */
 __device__ __forceinline__ uint4 ks_widen(uint32_t w, __half2 s, __half2 m) {
     const __half2 k1024 = ks_h2(0x64006400u), k16th = ks_h2(0x2C002C00u), k64 = ks_h2(0xD400D400u); /* 1024, 1 / 16, -64 */
@@ -440,8 +445,8 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 const int largest = (int)max(big & 0xFFFFu, big >> 16), e = largest ? min(136 - (largest >> 7), 120) : 0; /* 2^9 <= it times 2^e < 2^10 */
                 const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                 if (r < KS_ROWS) {
-                    if (u == 0) /* 2 log2(e) / sqrt(128) 2^-e */
-                        sh_factor[unit & 3][tile * KS_ROWS + r] = __uint_as_float((uint32_t)(127 - e) << 23) * (2.0f * 1.4426950408889634f * 0.08838834764831845f);
+                    if (u == 0) /* log2(e) / sqrt(128) 2^-e */
+                        sh_factor[unit & 3][tile * KS_ROWS + r] = __uint_as_float((uint32_t)(127 - e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
                     uint4 h; /* channels 0, 4, 1, 5, 2, 6, 3, 7 of the unit of eight, as ks_widen puts them */
                     h.x = ks_half2(bf_lo(w[k].x) * up, bf_lo(w[k].z) * up);
                     h.y = ks_half2(bf_hi(w[k].x) * up, bf_hi(w[k].z) * up);
@@ -581,7 +586,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     ks_ld32(t_o + 32 * c, v);
                     ks_ld_wait();
                     float y[32];
-                    const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 2.0f / sum; /* (the values' halves) */
+                    const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
                     for (int k = 0; k < 32; k++) y[k] = __uint_as_float(v[k]) * scale;
                     if (whole) {
@@ -635,10 +640,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 ok = ok && (turn == 0 || ks_wait_warp(&bars.k_free[stage], (turn - 1) & 1, status));
                 unsigned char* to = sk + stage * KS_K_BYTES;
                 if (ok) {
+                    bool wide = false;
 #pragma unroll 1
                     for (int j = 0; j < 2; j++) { /* this thread's units are in blocks p >> 6 and 2 + (p >> 6) */
                         const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
-                        const uint4 kc = *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16), kp = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16));
+                        const uint4 kc = *reinterpret_cast<const uint4*>(blk + plane * 512 + lane * 16), kp = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_K + (plane * 8 + g) * 16);
                         const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + g;
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
@@ -646,7 +652,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                             const __half2 sc = ks_h2(prmt(sw, sw, (k & 1) ? 0x3232 : 0x1010)), mn = ks_h2(prmt(mw, mw, (k & 1) ? 0x3232 : 0x1010));
                             *reinterpret_cast<uint4*>(to + (4 * k + t) * KS_K_PITCH + pos * 16) = ks_widen(ks_word(kc, k), sc, mn);
                         }
+                        wide |= ks_wide(kp);
                     }
+                    if (__builtin_expect(wide, 0))
+#pragma unroll 1
+                        for (int k = 0; k < 8; k++) ks_keep(to + (4 * (k & 3) + t) * KS_K_PITCH + ((k >> 2) * 32 + (p >> 6) * 16 + plane * 8 + g) * 16);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.k_full[stage]);
@@ -654,12 +664,13 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 ok = ok && (turn == 0 || ks_wait_warp(&bars.v_free[stage], (turn - 1) & 1, status));
                 to = sv + stage * KS_V_BYTES;
                 if (ok) {
-#pragma unroll
+                    bool wide = false;
+#pragma unroll 1
                     for (int j = 0; j < 2; j++) {
                         const unsigned char* blk = page + (2 * j + (p >> 6)) * KV4_BLOCK_BYTES;
                         const uint4 vc = *reinterpret_cast<const uint4*>(blk + 1024 + plane * 512 + lane * 16);
-                        const uint4 vs = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16)),
-                                    vm = ks_halve(*reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16));
+                        const uint4 vs = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + (plane * 4 + t) * 16),
+                                    vm = *reinterpret_cast<const uint4*>(blk + KV4_PARAMS_V + 128 + (plane * 4 + t) * 16);
                         const int pos = (2 * j + (p >> 6)) * 16 + plane * 8 + 2 * t;
 #pragma unroll
                         for (int k = 0; k < 4; k++) { /* positions pos, pos + 1; words of groups 0, 1 and 2, 3 */
@@ -672,7 +683,11 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                             if (absent || i * KS_TILE + pos + second >= s.seen) v = make_uint4(0, 0, 0, 0);
                             *reinterpret_cast<uint4*>(to + (g + 8 * word) * KS_V_PITCH + (pos + second) * 16) = v;
                         }
+                        wide |= ks_wide(vs) | ks_wide(make_uint4(vs.z, vs.w, 0, 0));
                     }
+                    if (__builtin_expect(wide, 0))
+#pragma unroll 1
+                        for (int k = 0; k < 8; k++) ks_keep(to + (g + 8 * (k & 1)) * KS_V_PITCH + ((k >> 2) * 32 + (p >> 6) * 16 + plane * 8 + 2 * t + (k >> 1 & 1)) * 16);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.v_full[stage]);
@@ -819,7 +834,7 @@ __global__ void __launch_bounds__(KS_JOIN_THREADS) k_kv4_join(KsParts parts, int
         }
         top = now;
     }
-    const float scale = sum == 0.0f ? 0.0f : 2.0f / sum; /* (the values' halves) */
+    const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
     __nv_bfloat16* to = out + ((size_t)(unit.x + row) * q_heads + unit.z * group + in % group) * 128 + 64 * (u >> 3) + 4 * (u & 7);
 #pragma unroll
     for (int odd = 0; odd < 2; odd++) {

@@ -15,6 +15,15 @@ def gauss(*shape, seed=0):
     return torch.randn(*shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda")
 
 
+def close(cache, entries, q, out):
+    """entries: (sequence, first position, first row, rows)."""
+    torch.cuda.synchronize()
+    for seq, first, r0, n in entries:
+        want, bound = _kv4.attention_close(cache, seq, first, q[r0:r0 + n])
+        off = (out[r0:r0 + n].double() - want).abs()
+        assert bool((off <= bound).all()), (seq, first, n, float((off / bound).max()), float((off.norm() / want.norm())))
+
+
 @pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (3, 3), (16, 1)])
 @pytest.mark.parametrize("first,rows", [(0, 1), (0, 130), (5, 1), (70, 3), (70, 100)])
 @pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
@@ -48,3 +57,42 @@ def test_a_query_that_is_not_finite_makes_its_head_nan(mine, capi, q_heads, kv_h
         cache.attention(b, q, out)
         torch.cuda.synchronize()
         assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("scale", [3e-7, 1e-6, 1e-5, 1e-4, 1e-3, 1.0, 1000.0])
+@pytest.mark.parametrize("what", ["keys", "values", "both"])
+@pytest.mark.parametrize("length,rows", [(130, 130), (2000, 70)])
+def test_keys_and_values_of_any_size_for_slices(mine, capi, scale, what, length, rows):
+    """s c + m has all the bits that the cache holds, down to f16's smallest numbers."""
+    cache = _kv4.Cache(mine, capi, 40, kv_heads=2, q_heads=8, stride=40, rows=rows)
+    ks, vs = (scale if what in (name, "both") else 1.0 for name in ("keys", "values"))
+    _kv4.store(cache, 0, gauss(2, length, 128, seed=1) * ks, gauss(2, length, 128, seed=2) * vs)
+    b = cache.batch([0], [rows], [length - rows])
+    q = (gauss(rows, 8 * 128, seed=3) * 1.5 / ks).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    close(cache, [(0, length - rows, 0, rows)], q, out)
+
+
+@pytest.mark.parametrize("rows", [1, 130])
+def test_groups_that_reach_beyond_f16(mine, capi, rows):
+    """The largest value of a group of the widest range is 65536, which f16 has not: it counts as 65504 at the least, the values beside it as they are."""
+    length = 200
+    cache = _kv4.Cache(mine, capi, 8, kv_heads=2, q_heads=8, stride=4, rows=rows)
+    v = gauss(2, length, 128, seed=2)
+    v[:, ::3] *= 1e6
+    v[:, 1::3, 32:64] *= 65504 / v[:, 1::3, 32:64].abs().amax(-1, keepdim=True)
+    top = 65504 - torch.rand(2, 66, 1, generator=torch.Generator("cuda").manual_seed(4), device="cuda").mul(11).exp()  # ranges of 1 to 60000 below the largest
+    v[:, 2:200:3, 96:] = top + (65504 - top) * torch.rand(2, 66, 32, generator=torch.Generator("cuda").manual_seed(5), device="cuda")
+    v[:, 2:200:3, 100] = 65504
+    v[:, 2:200:3, 101] = (top[..., 0] / 16).round() * 16
+    k = gauss(2, length, 128, seed=1)
+    k[:, ::5, 64:96] *= 1e6
+    _kv4.store(cache, 0, k, v)
+    b = cache.batch([0], [rows], [length - rows])
+    q = gauss(rows, 8 * 128, seed=3).view(rows, 8, 4, 32)
+    q[:, :, 2] *= 1e-5
+    q = q.reshape(rows, -1).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    close(cache, [(0, length - rows, 0, rows)], q, out)
