@@ -13,7 +13,8 @@
  *            value 512..1023 (exact: bf16 has 8 bits).  One accumulator per group, scaled by s in 32 bits; the m term is one more
  *            product, m times the sums of q split into two f16.
  *   softmax  running maximum and sum in 32 bits, base 2; the maximum is renewed only when a score passes it by 2, so that a
- *            block normally costs one vote.  p (at most 4) is rounded to f16, 11 bits, for the products.
+ *            block normally costs one vote.  The maximum is taken off before a score is scaled: the scaled one would be rounded, by thousands where queries are
+ *            large enough, and what is left of the largest score would then be an exponent that no f16 has.  p (at most 4) is rounded to f16, 11 bits, for the products.
  *   values   O^T [128 channels x columns]: A = values, the pairs of positions put together by byte permutation, B = p^T, which is
  *            S^T transposed in registers (movmatrix), times s of the group (rounded to f16 once more; at most 4 * 8734).
  *
@@ -160,8 +161,9 @@ __device__ __forceinline__ void ka_load_query(KaQuery<NT>& z, const __nv_bfloat1
 template <int NT> struct KaState {
     float o[NT][8][4]; /* [column tile][channel tile 2 j + h]: rows 4 g + 2 h (16 times 2^-24 that of the second) and + 1 of group j */
     float om[NT][4];   /* [0], [1], in lanes with g < 4: sum of p m of group g; [2], [3]: sum of p */
-    float max[NT][2];
+    float max[NT][2]; /* of the scores before they are scaled */
 };
+constexpr float KA_NONE = -1e38f; /* maximum of a column that has seen nothing: finite, so that weights relative to it are zero */
 template <int NT> __device__ __forceinline__ void ka_clear(KaState<NT>& z) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -171,8 +173,13 @@ template <int NT> __device__ __forceinline__ void ka_clear(KaState<NT>& z) {
             for (int r = 0; r < 4; r++) z.o[nt][i][r] = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; r++) z.om[nt][r] = 0.0f;
-        z.max[nt][0] = z.max[nt][1] = -INFINITY;
+        z.max[nt][0] = z.max[nt][1] = KA_NONE;
     }
+}
+
+/* what a column's sums are relative to, for those who put parts together */
+template <int NT> __device__ __forceinline__ float ka_base(const KaState<NT>& z, const KaQuery<NT>& q, int nt, int c) {
+    return z.max[nt][c] == KA_NONE ? -INFINITY : z.max[nt][c] * q.factor[nt][c];
 }
 
 /* Two blocks of 16 positions from shared memory: their instructions interleave.  Where `masked`, left(column tile, 0 or 1) says how many of the 32
@@ -240,7 +247,7 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
             float top = fmaxf(score[0][nt][c], score[0][nt][c + 2]);
 #pragma unroll
             for (int n = 1; n < NB; n++) top = fmaxf(top, fmaxf(score[n][nt][c], score[n][nt][c + 2]));
-            over |= top * q.factor[nt][c] > z.max[nt][c] + 2.0f;
+            over |= (top - z.max[nt][c]) * q.factor[nt][c] > 2.0f;
         }
     if (__any_sync(S2P_FULL_MASK, over)) {
 #pragma unroll
@@ -253,8 +260,8 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
                 top = fmaxf(top, __shfl_xor_sync(S2P_FULL_MASK, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(S2P_FULL_MASK, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(S2P_FULL_MASK, top, 16));
-                top = fmaxf(top * q.factor[nt][c], z.max[nt][c]);
-                const float shrink = top == -INFINITY ? 1.0f : ka_exp2(z.max[nt][c] - top);
+                top = fmaxf(top, z.max[nt][c]);
+                const float shrink = ka_exp2((z.max[nt][c] - top) * q.factor[nt][c]);
                 z.max[nt][c] = top;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -265,11 +272,6 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
                 z.om[nt][c + 2] *= shrink;
             }
     }
-    float base2[NT][2]; /* of columns that have seen nothing yet: a finite one */
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) base2[nt][c] = z.max[nt][c] == -INFINITY ? 0.0f : z.max[nt][c];
     uint32_t p[NB][NT][2];
 #pragma unroll
     for (int n = 0; n < NB; n++)
@@ -278,7 +280,7 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
             float e[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                e[r] = ka_exp2(fmaf(score[n][nt][r], q.factor[nt][r & 1], -base2[nt][r & 1]));
+                e[r] = ka_exp2((score[n][nt][r] - z.max[nt][r & 1]) * q.factor[nt][r & 1]);
             }
             p[n][nt][0] = ka_transpose(ka_half2(e[0], e[1]));
             p[n][nt][1] = ka_transpose(ka_half2(e[2], e[3]));
@@ -316,7 +318,7 @@ __device__ __forceinline__ void ka_blocks(KaState<NT>& z, const KaQuery<NT>& q, 
 /* Partial results: slot 2 w + 1 where worker w begins a unit that others end, 2 w where it goes on with one. */
 static_assert((size_t)KV4_PARTS * (128 + 2) * sizeof(float) <= KV4_AREA_BYTES, "the tokens' partials");
 struct KaParts {
-    float *max, *sum, *o; /* [slot][8 NT columns](, [128]) */
+    float *max, *sum, *o; /* [slot][8 NT columns](, [128]); max: ka_base */
     unsigned* arrived;    /* [row][kv head] of a unit's first row */
 };
 
@@ -663,7 +665,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
 #pragma unroll
                         for (int j = 0; j < 4; j++) *reinterpret_cast<float4*>(to + 32 * j) = channels(nt, c, j);
                         if (g == 0) {
-                            parts.max[slot * COLS + col] = z.max[nt][c];
+                            parts.max[slot * COLS + col] = ka_base(z, query, nt, c);
                             parts.sum[slot * COLS + col] = z.om[nt][2 + c];
                         }
                     }
@@ -721,7 +723,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
 #pragma unroll
                 for (int c = 0; c < 2; c++)
                     if (g == 0) {
-                        sh_max[warp][nt * 8 + 2 * t + c] = z.max[nt][c];
+                        sh_max[warp][nt * 8 + 2 * t + c] = ka_base(z, query, nt, c);
                         sh_sum[warp][nt * 8 + 2 * t + c] = z.om[nt][2 + c];
                     }
 #pragma unroll

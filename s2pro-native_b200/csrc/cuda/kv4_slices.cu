@@ -4,7 +4,8 @@
  * query heads of that kv head (32 rows at G = 4).  It walks the sequence page by page:
  *
  *   S = Q K^T    [128 x 64], tcgen05.mma, both operands in shared memory, f32 in TMEM
- *   P = 2^(S f - m), f16, over columns that held S; running maximum m and sum in 32 bits, m renewed where a score passes it by 8
+ *   P = 2^((S - m) f), f16, over columns that held S; running maximum m and sum in 32 bits, m renewed where a score passes it by 8.  (S f - m f, one instruction less a
+ *   pair, leaves the rounding of m f as the largest exponent: thousands where queries are large enough.)
  *   O += P V     [128 x 128], P from TMEM, V in shared memory, f32 in TMEM
  *
  * Roles, coupled by mbarriers only:
@@ -130,10 +131,10 @@ __device__ __forceinline__ float ks_exp2(float x) {
     return r;
 }
 /* two at a time; three at a time */
-__device__ __forceinline__ float2 ks_fma2(float2 a, float2 b, float2 c) {
+__device__ __forceinline__ float2 ks_mul2(float2 a, float2 b) {
     float2 d;
-    asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
 __device__ __forceinline__ float2 ks_add2(float2 a, float2 b) {
@@ -505,9 +506,9 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int k = 0; k < 64; k += 2) m4[(k >> 1) & 3] = ks_max3(m4[(k >> 1) & 3], __uint_as_float(v[k >> 5][k & 31]), __uint_as_float(v[k >> 5][(k + 1) & 31]));
-                    const float most = ks_max3(ks_max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * f;
-                    if (__any_sync(S2P_FULL_MASK, most > top + 8.0f)) {
-                        const float now = fmaxf(most, top), shrink = now == -INFINITY ? 1.0f : ks_exp2(top - now);
+                    const float most = ks_max3(ks_max3(m4[0], m4[1], m4[2]), m4[3], m4[3]);
+                    if (__any_sync(S2P_FULL_MASK, (most - top) * f > 8.0f)) {
+                        const float now = fmaxf(most, top), shrink = now == -INFINITY ? 1.0f : ks_exp2((top - now) * f);
                         top = now;
                         sum *= shrink;
                         if (i > s.t0) { /* behind the product of the page before; the one before that was waited for in front of these scores */
@@ -533,7 +534,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                         uint32_t p[16];
 #pragma unroll
                         for (int k = 0; k < 16; k++) {
-                            const float2 a = ks_fma2(make_float2(__uint_as_float(v[h][2 * k]), __uint_as_float(v[h][2 * k + 1])), f2, minus);
+                            const float2 a = ks_mul2(ks_add2(make_float2(__uint_as_float(v[h][2 * k]), __uint_as_float(v[h][2 * k + 1])), minus), f2);
                             const float2 w = make_float2(ks_exp2(a.x), ks_exp2(a.y));
                             s2[k & 1] = ks_add2(s2[k & 1], w);
                             p[k] = ks_half2(w.x, w.y);
@@ -598,7 +599,7 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
                 }
                 ks_before_sync(); /* the next unit's first product writes where this has been read */
                 if (!whole && live) {
-                    parts.max[slot * KS_SOFTMAX + tid] = top;
+                    parts.max[slot * KS_SOFTMAX + tid] = top == -INFINITY ? top : top * f; /* (without a page f is not there) */
                     parts.sum[slot * KS_SOFTMAX + tid] = sum;
                 }
             }

@@ -96,3 +96,26 @@ def test_groups_that_reach_beyond_f16(mine, capi, rows):
     out = torch.full_like(q, 7.0)
     cache.attention(b, q, out)
     close(cache, [(0, length - rows, 0, rows)], q, out)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e7, 1e10, 1e20, 1e29])
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 3000.0])
+def test_queries_that_see_one_key(mine, capi, size, scale, rows):
+    """Logits from 10^4 to 10^30, each row's along one key: that position's value comes out, and nothing leaves f16 on the way."""
+    length = 700
+    cache = _kv4.Cache(mine, capi, 12, kv_heads=1, q_heads=4, stride=12, rows=rows)
+    _kv4.store(cache, 0, gauss(1, length, 128, seed=1), gauss(1, length, 128, seed=2) * scale)
+    held = [torch.zeros(length, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    cache.read(cache.batch([0], [length], [0]), *held)
+    at = torch.randint(0, length - rows, (rows, 4), generator=torch.Generator().manual_seed(7)).cuda()
+    q = (held[0][at].float() * size).bfloat16().view(rows, -1)  # |k|^2 is about 128, other products at most 6 times 11
+    b = cache.batch([0], [rows], [length - rows])
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    torch.cuda.synchronize()
+    # the weight of any other is below e^(-size 60 / sqrt(128)); f16 twice and bf16 twice, the second for what is compared with
+    want = held[1][at].double().view(rows, -1)
+    off = (out.double() - want).abs()
+    top = want.abs().view(rows, 4, 128).amax(-1, keepdim=True).expand(-1, -1, 128).reshape(rows, -1)
+    assert bool((off <= want.abs() * 2 ** -7 * 1.01 + top * 2 ** -9).all()), float((off / top).max())
