@@ -174,8 +174,8 @@ s2p_status s2p_b200_kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
 
 /* out [rows, q_heads * 128]: softmax(q k / sqrt(128)) v over the positions of the row's sequence up to its own that have a
  * page; zeros where there is none.  out may be q.  Queries are below 2^100 in magnitude; a NaN or an infinity in a head's query
- * makes that head of the row NaN.  rows * kv_heads * table_stride is at most 2^29.  Scores, sums and results are in 32 bits; weights, and in the
- * kernel for slices keys and values s c + m, are rounded to f16 for the products, out to bf16.  That kernel's waits are bounded: see
+ * makes that head of the row NaN.  rows * kv_heads * table_stride is at most 2^29.  Scores, sums and results are in 32 bits; weights are rounded to
+ * f16 for the products, and so are the weights times s in the kernel for tokens, keys and values s c + m in the one for slices; out is rounded to bf16.  That kernel's waits are bounded: see
  * s2p_b200_kv4_status. */
 s2p_status s2p_b200_kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const s2p_bf16* q, s2p_bf16* out,
                                   cudaStream_t stream);

@@ -59,6 +59,36 @@ def test_a_query_that_is_not_finite_makes_its_head_nan(mine, capi, q_heads, kv_h
         assert bool((out == 0).all())
 
 
+@pytest.mark.parametrize("scale", [1e-5, 1e-4, 1e-3, 1e-2, 0.1, 10.0, 1000.0])
+@pytest.mark.parametrize("length,rows", [(40, 1), (3000, 1), (3000, 3), (16000, 1)])
+def test_values_of_any_size_for_tokens(mine, capi, scale, length, rows):
+    """The weights' products with s stay where f16 has all its bits."""
+    cache = _kv4.Cache(mine, capi, 260, kv_heads=2, q_heads=8, stride=256)
+    _kv4.store(cache, 0, gauss(2, length, 128, seed=1), gauss(2, length, 128, seed=2) * scale)
+    b = cache.batch([0], [rows], [length - rows])
+    q = (gauss(rows, 8 * 128, seed=3) * 1.5).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    close(cache, [(0, length - rows, 0, rows)], q, out)
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (16, 1)])
+@pytest.mark.parametrize("sizes", [(1e-3, 1.0, 20.0, 1.0), (1e-3, 100.0), (1.0, 300.0, 1e4), (1e4, 1e-3), (1e-4, 1e-3, 1e-2, 0.1, 1.0, 10.0, 100.0, 1000.0)])
+def test_values_whose_size_changes_along_a_sequence(mine, capi, sizes, rows, q_heads, kv_heads):
+    """What has been summed is carried over when s outgrows what the weights were scaled for; the groups of a head differ by a factor of 16 besides."""
+    length = 2300
+    cache = _kv4.Cache(mine, capi, 40, kv_heads=kv_heads, q_heads=q_heads, stride=40)
+    grow = torch.tensor(sizes, device="cuda").repeat_interleave(-(-length // len(sizes)))[:length, None]
+    v = gauss(kv_heads, length, 128, seed=2) * grow * torch.tensor([1.0, 4.0, 0.25, 2.0], device="cuda").repeat_interleave(32)
+    _kv4.store(cache, 0, gauss(kv_heads, length, 128, seed=1), v)
+    b = cache.batch([0], [rows], [length - rows])
+    q = (gauss(rows, q_heads * 128, seed=3) * 1.5).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    close(cache, [(0, length - rows, 0, rows)], q, out)
+
+
 @pytest.mark.parametrize("scale", [3e-7, 1e-6, 1e-5, 1e-4, 1e-3, 1.0, 1000.0])
 @pytest.mark.parametrize("what", ["keys", "values", "both"])
 @pytest.mark.parametrize("length,rows", [(130, 130), (2000, 70)])
