@@ -159,9 +159,9 @@ size_t s2p_b200_kv4_work_bytes(const s2p_b200_kv4* c, int rows);
 s2p_status s2p_b200_kv4_status(const s2p_b200_kv4* c, cudaStream_t stream);
 
 /* Room for the batch's rows: pos0 = positions held, lens += rows, and free pages (lowest first, in the batch's order) for
- * what the last held page does not take.  An entry that needs more pages than are left after all before it, or more table
- * entries than there are, or whose sequence stands in the batch before it, is refused: pos0 = -1, and it keeps what it held.  info (device, may be NULL): pages free
- * afterwards, entries refused. */
+ * what the last held page does not take.  An entry that needs more pages than all before it leave (those of refused ones count, so
+ * that none goes ahead of them), or more table entries than there are, or whose sequence stands in the batch before it, is refused: pos0 = -1, and it keeps
+ * what it held.  info (device, may be NULL): pages free afterwards, entries refused. */
 s2p_status s2p_b200_kv4_reserve(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int32_t* info, cudaStream_t stream);
 
 /* From raw rows qkv [rows, (q_heads + 2 kv_heads) * 128]: RMS norm of each query and key head (gains q_norm, k_norm [128];

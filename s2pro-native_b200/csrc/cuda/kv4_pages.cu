@@ -27,29 +27,29 @@ static inline Kv4Lists kv4_lists(const s2p_b200_kv4& c) {
 }
 
 /* sum over all threads before this one; the total to `total`.  Every thread of the CTA calls it. */
-__device__ __forceinline__ int kv4_scan(int v, int& total, int* sh) {
+template <class T> __device__ __forceinline__ T kv4_scan(T v, T& total, T* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int incl = v;
+    T incl = v;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(S2P_FULL_MASK, incl, off);
+        const T o = __shfl_up_sync(S2P_FULL_MASK, incl, off);
         if (lane >= off) incl += o;
     }
     if (lane == 31) sh[warp] = incl;
     __syncthreads();
     if (warp == 0) {
-        const int w = sh[lane];
-        int wi = w;
+        const T w = sh[lane];
+        T wi = w;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int o = __shfl_up_sync(S2P_FULL_MASK, wi, off);
+            const T o = __shfl_up_sync(S2P_FULL_MASK, wi, off);
             if (lane >= off) wi += o;
         }
         sh[lane] = wi - w;
         if (lane == 31) sh[32] = wi;
     }
     __syncthreads();
-    const int before = sh[warp] + incl - v;
+    const T before = sh[warp] + incl - v;
     total = sh[32];
     __syncthreads();
     return before;
@@ -99,7 +99,8 @@ __device__ __forceinline__ int kv4_held(const Kv4Book& k, int seq) {
 }
 
 __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_reserve(Kv4Book k, s2p_b200_kv4_batch b, int32_t* info) {
-    __shared__ int sh[33], upto[S2P_B200_KV4_MAX_BATCH], first_of[S2P_B200_KV4_MAX_BATCH], seq_of[S2P_B200_KV4_MAX_BATCH];
+    __shared__ long long wide[33], upto[S2P_B200_KV4_MAX_BATCH]; /* 1024 entries may ask for 2^24 pages each */
+    __shared__ int sh[33], first_of[S2P_B200_KV4_MAX_BATCH], seq_of[S2P_B200_KV4_MAX_BATCH];
     constexpr int SLOTS = 2 * S2P_B200_KV4_MAX_BATCH;
     __shared__ int named[SLOTS], first_named[SLOTS]; /* the sequences that stand in the batch, and where first */
     const int e = threadIdx.x;
@@ -110,8 +111,8 @@ __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_reserve(Kv4Book k, s2p
     __syncthreads();
     grid_wait();
     grid_release();
-    int seq = -1, held = 0, need = 0, fits = 0, slot = 0;
-    long long after = 0;
+    int seq = -1, held = 0, fits = 0, slot = 0;
+    long long after = 0, need = 0;
     if (e < b.n) {
         seq = b.seqs[e];
         if ((unsigned)seq < (unsigned)k.max_seqs) {
@@ -126,11 +127,11 @@ __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_reserve(Kv4Book k, s2p
             held = kv4_held(k, seq);
             after = (long long)held + max(0, min(b.row0[e + 1], b.rows) - max(b.row0[e], 0));
             fits = after <= (long long)k.stride * S2P_B200_KV4_PAGE;
-            need = (int)min((after + S2P_B200_KV4_PAGE - 1) / S2P_B200_KV4_PAGE - kv4_pages_of(held), (long long)(1 << 20)); /* summed over 1024 */
+            need = (after + S2P_B200_KV4_PAGE - 1) / S2P_B200_KV4_PAGE - kv4_pages_of(held);
         }
     }
-    int total;
-    const int before = kv4_scan(need, total, sh);
+    long long total;
+    const long long before = kv4_scan(need, total, wide);
     const int n_free = total > 0 || info ? kv4_count_free(k.refs, k.n_pages, sh) : 0;
     const int given = fits && (need == 0 || before + need <= n_free);
     if (e < b.n) {
@@ -139,16 +140,16 @@ __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_reserve(Kv4Book k, s2p
         seq_of[e] = given ? seq : -1;
     }
     int n_given;
-    kv4_scan(given ? need : 0, n_given, sh); /* (its barriers also publish the arrays) */
+    kv4_scan(given ? (int)need : 0, n_given, sh); /* (its barriers also publish the arrays) */
     if (n_given > 0) {
-        kv4_each_free(k.refs, k.n_pages, min(total, n_free), sh, [&](int rank, int page) {
+        kv4_each_free(k.refs, k.n_pages, (int)min(total, (long long)n_free), sh, [&](int rank, int page) {
             int lo = 0, hi = b.n - 1; /* the first entry with upto > rank: its pages are those ranks */
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
                 if (upto[mid] > rank) hi = mid; else lo = mid + 1;
             }
             if (seq_of[lo] < 0) return;
-            const int step = rank - (lo ? upto[lo - 1] : 0);
+            const int step = rank - (lo ? (int)upto[lo - 1] : 0);
             k.table[(size_t)seq_of[lo] * k.stride + first_of[lo] + step] = page;
             k.refs[page] = 1;
         });
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_reserve(Kv4Book k, s2p
         if (given) k.lens[seq] = (int)after;
     }
     int refused;
-    kv4_scan(e < b.n && !given, refused, sh);
+    kv4_scan<int>(e < b.n && !given, refused, sh);
     if (info && e == 0) {
         info[0] = n_free - n_given;
         info[1] = refused;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_fork(Kv4Book k, Kv4For
         tail_to[e] = -1;
     }
     int n_need, n_given, refused;
-    const int rank = kv4_scan(from >= 0, n_need, sh);
+    const int rank = kv4_scan<int>(from >= 0, n_need, sh);
     if (from >= 0) taker[rank] = e;
     const int n_free = kv4_count_free(k.refs, k.n_pages, sh);
     if (n_need > 0) /* taker is published by the count's barriers */
@@ -228,13 +229,13 @@ __global__ void __launch_bounds__(KV4_SCAN_THREADS) k_kv4_fork(Kv4Book k, Kv4For
         full_of[e] = given ? full : 0;
         k.lens[list.child[e]] = given ? tokens : 0;
     }
-    const int at = kv4_scan(given && from >= 0, n_given, sh);
+    const int at = kv4_scan<int>(given && from >= 0, n_given, sh);
     if (given && from >= 0) {
         lists.moves[at] = make_int2(from, tail_to[e]);
         k.table[(size_t)list.child[e] * k.stride + full] = tail_to[e];
         k.refs[tail_to[e]] = 1;
     }
-    kv4_scan(e < n && !given, refused, sh);
+    kv4_scan<int>(e < n && !given, refused, sh);
     for (int i = warp; i < n; i += KV4_SCAN_WARPS) {
         const int32_t* source = k.table + (size_t)list.parent[i] * k.stride;
         int32_t* to = k.table + (size_t)list.child[i] * k.stride;

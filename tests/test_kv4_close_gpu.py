@@ -128,6 +128,36 @@ def test_groups_that_reach_beyond_f16(mine, capi, rows):
     close(cache, [(0, length - rows, 0, rows)], q, out)
 
 
+# ---- pages --------------------------------------------------------------------------------------------------------------------
+
+def test_reserve_of_more_pages_than_two_to_the_twentieth(mine, capi):
+    """All of them are given, or none."""
+    n_pages, need = 2 ** 20 + 100, 2 ** 20 + 5
+    cache = _kv4.Cache(mine, capi, 1, kv_heads=1, q_heads=1, max_seqs=3, stride=2 ** 20 + 200, rows=1)
+    pool = torch.empty(n_pages * _kv4.BLOCK * 4, dtype=torch.uint8, device="cuda")
+    cache.refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+    cache.c.pages, cache.c.refs, cache.c.n_pages = pool.data_ptr(), cache.refs.data_ptr(), n_pages
+    for seqs, counts, pos0, info in (([0, 1, 2], [64 * need, 64 * 95, 1], [0, 0, -1], [0, 1]),       # all pages there are, and one more
+                                     ([0], [64 * (n_pages + 1)], [-1], [n_pages, 1]),                 # more than the pool has
+                                     ([0, 1], [64 * (n_pages - 1), 65], [0, -1], [1, 1]),
+                                     ([0, 1], [64 * n_pages - 63, 0], [0, 0], [0, 0])):
+        cache.refs.zero_()
+        cache.table.fill_(-1)
+        cache.lens.zero_()
+        b = cache.batch(seqs, counts)
+        cache.reserve(b)
+        torch.cuda.synchronize()
+        assert b.pos0.cpu().tolist() == pos0 and cache.info.cpu().tolist() == info
+        at = 0
+        for s, c, p in zip(seqs, counts, pos0):
+            given = -(-c // 64) if p >= 0 else 0
+            assert int(cache.lens[s]) == (c if p >= 0 else 0)
+            assert torch.equal(cache.table[s, :given], torch.arange(at, at + given, dtype=torch.int32, device="cuda"))
+            assert bool((cache.table[s, given:] == -1).all())
+            at += given
+        assert int(cache.refs.sum()) == at and bool((cache.refs[:at] == 1).all())
+
+
 @pytest.mark.parametrize("rows", [1, 3, 40])
 @pytest.mark.parametrize("size", [1e3, 1e5, 1e7, 1e10, 1e20, 1e29])
 @pytest.mark.parametrize("scale", [1e-3, 1.0, 3000.0])
