@@ -692,6 +692,7 @@ k_kv4_attn(Kv4View cache, Kv4Rows b, int few, int group, int rows_per, const __n
                 int last = 0;
                 if (lane == 0) last = kv4_arrive(arrived, w1 - w0);
                 if (__shfl_sync(S2P_FULL_MASK, last, 0)) {
+                    __syncwarp(); /* what lane 0 has acquired, for all: a shuffle does not order memory */
                     for (int base = 0; base < columns; base += KA_PASS) {
                         float top[KA_PASS], sum[KA_PASS];
                         float4 acc[KA_PASS];

@@ -128,6 +128,24 @@ def test_groups_that_reach_beyond_f16(mine, capi, rows):
     close(cache, [(0, length - rows, 0, rows)], q, out)
 
 
+# ---- parts --------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lens", [[32000], [32000, 9000], [700, 640, 650, 700, 690, 610, 500, 700, 100], [6000] + [90, 100, 1, 64] * 4, [500, 513, 480, 511] * 7,
+                                  [2100, 300, 64, 1, 1700, 900, 17, 3000] * 3, [33, 70, 1, 16, 128, 64, 99, 130] * 20])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (16, 1), (32, 8)])
+def test_no_part_of_a_sequence_is_lost_for_tokens(mine, capi, lens, q_heads, kv_heads):
+    """Weights that hardly differ, so that every part, piece and page counts alike: one of 500 that is left out is off by several bounds."""
+    n = len(lens)
+    cache = _kv4.Cache(mine, capi, sum((x + 63) // 64 for x in lens) + 1, kv_heads=kv_heads, q_heads=q_heads, max_seqs=n, stride=512, rows=n)
+    for i, x in enumerate(lens):
+        _kv4.store(cache, i, gauss(kv_heads, x, 128, seed=2 * i), gauss(kv_heads, x, 128, seed=2 * i + 1))
+    b = cache.batch(range(n), [1] * n, [x - 1 for x in lens])
+    q = (gauss(n, q_heads * 128, seed=9) * 0.3).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    close(cache, [(i, x - 1, i, 1) for i, x in enumerate(lens)], q, out)
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------
 
 def test_reserve_of_more_pages_than_two_to_the_twentieth(mine, capi):
