@@ -146,6 +146,26 @@ def test_no_part_of_a_sequence_is_lost_for_tokens(mine, capi, lens, q_heads, kv_
     close(cache, [(i, x - 1, i, 1) for i, x in enumerate(lens)], q, out)
 
 
+@pytest.mark.parametrize("lens,counts", [([7000], [700]), ([7000], [65]), ([1000], [1000]), ([7000] + [50] * 12, [32] + [40] * 12), ([300, 250, 333], [70, 64, 65]),
+                                         ([4000, 3900], [300, 290]), ([1500] * 16, [1] * 15 + [512]), ([64, 500, 129, 700] * 4, [64, 100, 128, 33] * 4)])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (16, 1), (32, 8)])
+def test_no_part_of_a_sequence_is_lost_for_slices(mine, capi, lens, counts, q_heads, kv_heads):
+    n, total = len(lens), sum(counts)
+    cache = _kv4.Cache(mine, capi, sum((x + 63) // 64 for x in lens) + 1, kv_heads=kv_heads, q_heads=q_heads, max_seqs=n, stride=128, rows=total)
+    for i, x in enumerate(lens):
+        _kv4.store(cache, i, gauss(kv_heads, x, 128, seed=2 * i), gauss(kv_heads, x, 128, seed=2 * i + 1))
+    b = cache.batch(range(n), counts, [x - c for x, c in zip(lens, counts)])
+    q = (gauss(total, q_heads * 128, seed=9) * 0.3).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attention(b, q, out)
+    entries = []
+    for i, (x, c) in enumerate(zip(lens, counts)):
+        for r in range(0, c, 128):  # (a few rows at a time: the weights are in 64 bits)
+            m = min(128, c - r)
+            entries.append((i, x - c + r, sum(counts[:i]) + r, m))
+    close(cache, entries, q, out)
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------
 
 def test_reserve_of_more_pages_than_two_to_the_twentieth(mine, capi):
