@@ -176,7 +176,9 @@ s2p_status s2p_b200_kv4_append(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* 
  * page; zeros where there is none.  out may be q.  Queries are below 2^100 in magnitude; a NaN or an infinity in a head's query
  * makes that head of the row NaN.  rows * kv_heads * table_stride is at most 2^29.  Scores, sums and results are in 32 bits; weights are rounded to
  * f16 for the products, and so are the weights times s in the kernel for tokens, keys and values s c + m in the one for slices; out is rounded to bf16.  That kernel's waits are bounded: see
- * s2p_b200_kv4_status. */
+ * s2p_b200_kv4_status.  Slices have it as long as the batch's work fits its list: rows / (2 (128 / group)) + 5 n up to about 4660, group = q_heads / kv_heads (one sequence up to
+ * 298 thousand rows at four query heads to a kv head, 900 entries with 10 thousand).  Beyond that the kernel for tokens takes the whole batch, several times slower for long
+ * slices: split such a batch. */
 s2p_status s2p_b200_kv4_attention(const s2p_b200_kv4* c, const s2p_b200_kv4_batch* b, int layer, const s2p_bf16* q, s2p_bf16* out,
                                   cudaStream_t stream);
 

@@ -84,9 +84,9 @@ __device__ __forceinline__ uint32_t kv4_quantise(float (&v)[8], unsigned half, _
     s_out = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
     m_out = __float2half_rn(lo);
     const float s = __half2float(s_out), m = __half2float(m_out), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
-    /* To the nearest whole number, ties to even, by adding 2^23 + 2^22, which leaves it in the low bits.  A quotient by way of the reciprocal is off by
-     * less than 1e-5 (it is at most 16 and a bit, three roundings), so it rounds to the same code unless it lies that close to the middle
-     * between two: then it is divided after all. */
+    /* To the nearest whole number, ties to even, by adding 2^23 + 2^22, which leaves it in the low bits.  A quotient by way of the reciprocal
+     * has three roundings.  Without a limit it may be large (m is rounded: with 1000.30 the least and a range of 0.01 it is -300), but where it is kept at 0 or 15 the divided
+     * one is too, and up to 15 it is off by less than 1e-5: it rounds to the same code unless it lies that close to the middle between two.  Then it is divided after all. */
     const float big = 12582912.0f;
     uint32_t codes = 0;
     float t[8], off = 0.0f;

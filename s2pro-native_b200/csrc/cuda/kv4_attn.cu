@@ -35,17 +35,22 @@ constexpr int KA_PASS = 4;                                         /* columns me
 constexpr int KA_MERGE_BYTES = KA_WARPS * KA_PASS * 128 * 4;
 constexpr int KA_LEAST_CTA = KA_WARPS, KA_LEAST_WARP = 8;          /* blocks that make a worker worth its while */
 /* (Row, head) columns of a kv head up to which an entry is this kernel's rather than that of the tensor cores: alone, and next to longer slices, where
- * most bring a token.  us here and there, 32 query and 8 kv heads: 4, 8, 16, 32 rows of one sequence of 1100 positions 17.4, 18.8, 18.6, 19.9 and 17.6, 17.8,
- * 18.3, 19.2; of 8000 positions 20.4, 22.3, 28.1, 48.9 and 24.0, 25.0, 25.8, 27.7; 4, 8 rows of 16 sequences of 4000 41.5, 53.9 and 80, 81. */
+ * most bring a token.  us here and there, 32 query and 8 kv heads (8 and 8 the same by columns), 32, 36, 48, 64 columns:
+ *   one sequence of  500     12.0 12.0 12.1 12.1 and 16.8 16.9 16.9 17.2      16 of 1000  27 30 31 36 and 34 35 35 35
+ *                   1100     18.7 16.8 17.0 18.4 and 18.1 18.2 18.3 18.7      16 of 4000  62 73 73 97 and 78 82 82 82
+ *                   8000     21.9 24.2 24.3 27.6 and 25.4 25.5 25.5 26.9      64 of 300   22 46 46 53 and -- 68 68 69
+ *                  20000     29.1 72.2 76.6 68.9 and   --  36.6 36.5 38.0
+ * The crossing goes by the context, which the host does not know: 64 is the better side for short and medium ones, and costs up to twice the time for one long sequence. */
 constexpr int KA_FEW = 64, KA_FEW_BESIDE = 32;
 /* How the work is cut (us, 32 query and 8 kv heads, one row a sequence).  Units each cut into equal parts, one to a CTA, its warps joined through shared memory,
- * wherever there are no more units than CTAs: 15 sequences of 1500 13.0, by warps below 20.6; up to KA_LONG blocks to a warp, where the warps' barriers cost more
+ * wherever there are no more units than CTAs: 15 sequences of 1500 13.3, by warps below 20.6; up to KA_LONG blocks to a warp, where the warps' barriers cost more
  * than the partials that they save (9 of 8000 28.2 and 27.5, 12 of 4000 24.0 and 22.8), and where no part has KA_SECOND blocks more than an equal share (one
  * sequence of 2000 among 15 of 1000, 67 more: 14.6 and 16.4; of 3000, 130 more: 18.2 and 17.8).  Units of up to KA_WHOLE blocks are not cut even so, since putting
  * parts together takes longer than more blocks do (one sequence of 512 whole 7.8, cut 9.0; 8 of 1000 11.0 and 12.0, of 1250 11.7 and 12.0; one of 1000 9.9 and 9.6, of
  * 1100 10.9 and 9.7).  Otherwise a warp is a worker by itself and leaves a partial.
  * Equal parts of each unit again (64 of 512: 18.0, 24 of 2500: 23.5), unless a part has KA_SECOND_WARP blocks more than an equal stretch of the line of all units'
- * blocks, in which many warps end one unit and begin the next (64 of 512 20.5, 24 of 2500 26.2; but 32 of 8192, 18 more: 58.5, in parts 66). */
+ * blocks, in which many warps end one unit and begin the next (64 of 512 20.5, 24 of 2500 26.2; but 32 of 8192, 18 more: 58.5, in parts 66).  (Taken before weights were
+ * lifted, which adds 1 to 2% on either side.) */
 constexpr int KA_SECOND = 120, KA_SECOND_WARP = 8, KA_LONG = 20, KA_WHOLE = 64;
 
 struct KaBatch { /* in shared memory, [n (+ 1)] */

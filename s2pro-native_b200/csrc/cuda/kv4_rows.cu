@@ -6,8 +6,9 @@
  * lanes.  All of it is in 32 bits up to the one rounding of the result; the angle is reduced in 64 (at position 32768 the fastest pair has
  * turned 5215 times: 32 bits would leave it 2e-3 off).
  *
- * Few rows are bound by latency (32 query and 8 kv heads, 1 to 32 rows: 7.2 to 7.4 us, launch included), many by the issue of instructions: 2055 rows 22 us, 56 MB in
- * that time, 60% of the issue slots busy; with a warp to a vector, 193 instructions each, 41 us. */
+ * Few rows are bound by latency (32 query and 8 kv heads, append and read of 1 to 32 rows: 7.2 us, launches included), many by the issue of instructions: append of 2055 rows,
+ * 44.7 MB, 18.9 us, of which HBM would take 6.9; 60% of the issue slots are busy.  (With a warp to a vector, 193 instructions each, append and read 41 us; now 25.8.)  Read of 2055
+ * rows, 11 MB, 8.9 us.  The row grid below was measured on the two together. */
 #include <math.h>
 #include "kv4.cuh"
 

@@ -22,11 +22,11 @@
  *
  * The pages of all units, and what each costs besides, form one line, and each CTA takes an equal stretch of it, wherever that cuts units.  With no more units than CTAs
  * most CTAs would get the end of one unit and the start of the next: there every unit is cut into equal parts of its own, one to a CTA
- * (32 query and 8 kv heads, 512 rows behind 1500: 49 -> 41 us, 77 behind 1024: 30 -> 24.5).  The parts of a
+ * (32 query and 8 kv heads, 512 rows behind 1500: 49 -> 41 us when it came, 39.4 now; 77 behind 1024: 30 -> 24.5).  The parts of a
  * unit are added, in order, by a second kernel over all SMs: in the last CTA to arrive that took 8 us for two parts of 128 KB and 20 for
  * five, with the other SMs idle.  Parts stay in 32 bits (f16 would take 1.5 us off the smallest calls).
- * A page takes a CTA 2100 cycles (2048 rows, the last of 8100, 32 query and 8 kv heads: 277 to 304 us at 1.75 to 1.6 GHz, 830 TFLOP/s); the tensor cores are busy 57% of
- * that, the issue slots 59%: the roles wait for each other's results. */
+ * A page takes a CTA 2180 cycles (2048 rows, the last of 8100, 32 query and 8 kv heads: 280 to 306 us at 1.75 to 1.6 GHz, 780 to 850 TFLOP/s); the tensor cores are busy 56% of
+ * that, the issue slots 63%: the roles wait for each other's results.  ptxas spills 64 bytes (260 loaded) at 96 registers. */
 #include "kv4.cuh"
 #include "pipe.cuh"
 
@@ -176,7 +176,7 @@ __device__ __forceinline__ uint4 ks_widen(uint32_t w, __half2 s, __half2 m) {
 }
 __device__ __forceinline__ uint32_t ks_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-/* Entries of up to `few` rows are left to the kernel for single tokens.  shift: registers of the row's place in a tile. */
+/* Entries of up to `few` rows are left to the kernel for single tokens. */
 __global__ void __launch_bounds__(KS_THREADS, 1)
 k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfloat16* out, KsParts parts) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -388,39 +388,39 @@ k_kv4_slices(Kv4View cache, Kv4Rows b, int few, const __nv_bfloat16* q, __nv_bfl
     };
 
     const int team = (warp >> 2) & 1, p = tid & 127;
-            /* The teams of warps 8..11 and 12..15: what to bring, a walk along the stretch of its own along the stretch, one page of the team ahead of the conversion */
-            unsigned f_cur = begin, f_it = 0;
-            int f_chunk = chunk_at, f_i = 0, page_of = -1; /* lane i keeps the (32 n + i)-th page of the segment */
-            Segment f;
-            f.t0 = f.t1 = 0;
-            auto bring = [&]() { /* the team's next page */
-                for (;;) {
-                    if (f_i == f.t1 - f.t0) {
-                        if (f_cur == end) break;
-                        f = segment(f_cur, f_chunk);
-                        f_cur = f.next;
-                        f_i = 0;
-                    }
-                    if ((f_i & 31) == 0) {
-                        const int pos = (f.t0 + f_i + lane) * S2P_B200_KV4_PAGE;
-                        page_of = f_i + lane < f.t1 - f.t0 && pos < f.seen ? kv4_page(cache, f.seq, pos) : -1;
-                    }
-                    const int page = __shfl_sync(S2P_FULL_MASK, page_of, f_i & 31);
-                    const unsigned now = f_it++;
-                    f_i++;
-                    if ((int)(now & 1) != team) continue;
-                    if (page >= 0) {
-                        const unsigned char* src = kv4_block(cache, page, f.head, 0) + p * 16;
-                        const uint32_t dst = smem_u32(raw) + (team * KS_RAW + now / 2 % KS_RAW) * KV4_HEAD_BYTES + p * 16;
-    #pragma unroll
-                        for (int k = 0; k < KV4_HEAD_BYTES / 2048; k++)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 2048), "l"(src + k * 2048) : "memory");
-                    }
-                    if (p == 0) sh_absent[now & 15] = page < 0;
-                    break;
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
+    /* The teams of warps 8..11 and 12..15: each walks along the stretch and brings its pages, one of its own ahead of the conversion. */
+    unsigned f_cur = begin, f_it = 0;
+    int f_chunk = chunk_at, f_i = 0, page_of = -1; /* lane i keeps the (32 n + i)-th page of the segment */
+    Segment f;
+    f.t0 = f.t1 = 0;
+    auto bring = [&]() { /* the team's next page */
+        for (;;) {
+            if (f_i == f.t1 - f.t0) {
+                if (f_cur == end) break;
+                f = segment(f_cur, f_chunk);
+                f_cur = f.next;
+                f_i = 0;
+            }
+            if ((f_i & 31) == 0) {
+                const int pos = (f.t0 + f_i + lane) * S2P_B200_KV4_PAGE;
+                page_of = f_i + lane < f.t1 - f.t0 && pos < f.seen ? kv4_page(cache, f.seq, pos) : -1;
+            }
+            const int page = __shfl_sync(S2P_FULL_MASK, page_of, f_i & 31);
+            const unsigned now = f_it++;
+            f_i++;
+            if ((int)(now & 1) != team) continue;
+            if (page >= 0) {
+                const unsigned char* src = kv4_block(cache, page, f.head, 0) + p * 16;
+                const uint32_t dst = smem_u32(raw) + (team * KS_RAW + now / 2 % KS_RAW) * KV4_HEAD_BYTES + p * 16;
+#pragma unroll
+                for (int k = 0; k < KV4_HEAD_BYTES / 2048; k++)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * 2048), "l"(src + k * 2048) : "memory");
+            }
+            if (p == 0) sh_absent[now & 15] = page < 0;
+            break;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     /* The query rows of a unit from row tile `tile`, a row to half a warp (a lane has 16 bytes of it), eight rows' loads under way; `first` and `step`:
      * what rows are this half warp's. */
     const unsigned by_group = (65536u + (unsigned)group - 1) / (unsigned)group; /* r / group = r by_group >> 16 for r < 128 */
