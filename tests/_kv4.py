@@ -2,6 +2,7 @@
 
 Everything here is written from the layout that include/s2p_b200_ext.h documents, with no code of the library."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -182,6 +183,11 @@ def attention(cache, seq, first, q, layer=0):
     return out.reshape(rows, -1), bound.reshape(rows, -1) + out.abs().reshape(rows, -1) * 2 ** -8
 
 
+@functools.lru_cache(None)
+def places_on(device, which):
+    return tuple(t.to(device) for t in places(which))
+
+
 def store(cache, seq, keys, values, layer=0):
     """Gives a sequence keys and values [kv_heads, length, 128] in free pages of a random order; positions behind the length keep what was there."""
     heads, length, _ = keys.shape
@@ -194,7 +200,7 @@ def store(cache, seq, keys, values, layer=0):
     flat, half = cache.pages[:, layer].view(-1), cache.pages[:, layer].view(-1).view(torch.float16)
     assert flat.data_ptr() == cache.pages.data_ptr()  # (caches of one layer)
     for which, x in ((0, keys), (1, values)):
-        byte, _, at_s, at_m = (t.to(dev)[place] for t in places(which))
+        byte, _, at_s, at_m = (t[place] for t in places_on(dev, which))
         codes, s, m = quantise(x.to(dev).float())
         for h in range(heads):
             base = (((page * heads + h) * 4 + block) * BLOCK)[:, None]
@@ -222,7 +228,7 @@ def attention_close(cache, seq, first, q, lift=12, layer=0):
     half = blocks.view(torch.float16)
     held = []
     for which in (0, 1):
-        byte, shift, s, m = (t.to(dev) for t in places(which))
+        byte, shift, s, m = places_on(dev, which)
         parts = [((blocks[..., byte] >> shift.to(torch.uint8)) & 15).double(), half[..., s // 2].double(), half[..., m // 2].double()]
         parts = [t.permute(1, 0, 2, 3, 4).reshape(heads, n * PAGE, 128)[:, :length] for t in parts]
         held += [torch.where(there[None, :, None], t, 0.0) for t in (parts[1] * parts[0] + parts[2], parts[1] * parts[0] + parts[2].abs(), parts[1])]
